@@ -14,6 +14,7 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libd
 F16, BF16, F32 = 0, 1, 2
 
 c_void_p, c_int, c_int64, c_float = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
+c_double = ctypes.c_double
 
 
 class Nf4Job(ctypes.Structure):
@@ -108,6 +109,28 @@ SIGNATURES = {
     "decik_varlen_attn_bwd_noalloc": (c_int, [Tensor3, Tensor3, Tensor3, Tensor3, Tensor3, c_void_p, Tensor3,
                                               Tensor3, Tensor3, c_void_p, c_int, c_int, c_int64, c_int, c_int, c_int,
                                               c_float, c_int, c_void_p]),
+    "decik_dropout": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int, c_int64, c_double, c_void_p, c_int64,
+                              c_void_p]),
+    "decik_lora_down_dropout": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                                        c_int64, c_int64, c_int, c_int, c_int, c_double, c_double, c_void_p, c_int64,
+                                        c_int, c_void_p]),
+    "decik_lora_down_dropout_bwd_workspace": (c_int64, [c_int64, c_int, c_int, c_int]),
+    "decik_lora_down_dropout_bwd": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64,
+                                            c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_int, c_double,
+                                            c_double, c_void_p, c_int64, c_int, c_void_p, c_void_p]),
+    "decik_qk_norm_rope_fwd": (c_int, [Tensor3, Tensor3, Tensor3, c_void_p, c_void_p, c_int, c_float, c_void_p,
+                                       c_void_p, Tensor3, Tensor3, c_int64, c_int, c_int, c_int, c_int, c_int,
+                                       c_void_p]),
+    "decik_qk_norm_rope_bwd_workspace": (c_int64, [c_int]),
+    "decik_qk_norm_rope_bwd": (c_int, [Tensor3, Tensor3, Tensor3, Tensor3, Tensor3, c_void_p, c_void_p, c_int, c_float,
+                                       c_void_p, c_void_p, Tensor3, Tensor3, c_void_p, c_void_p, c_int64, c_int,
+                                       c_int, c_int, c_int, c_int, c_void_p, c_void_p]),
+    "decik_rope_axes_fwd": (c_int, [Tensor3, Tensor3, Tensor3, c_void_p, c_void_p, c_int, c_float, c_void_p, c_int,
+                                    c_int64, c_int, c_void_p, c_void_p, Tensor3, Tensor3, c_int64, c_int, c_int, c_int,
+                                    c_int, c_int, c_void_p]),
+    "decik_rope_axes_bwd": (c_int, [Tensor3, Tensor3, Tensor3, Tensor3, Tensor3, c_void_p, c_void_p, c_int, c_float,
+                                    c_void_p, c_int, c_int64, c_int, c_void_p, c_void_p, Tensor3, Tensor3, c_void_p,
+                                    c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p]),
 }
 
 _lib = None

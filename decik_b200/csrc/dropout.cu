@@ -1,0 +1,78 @@
+// Dropout from a counter-based generator (philox.cuh), with no stored mask: out = [residual +]
+// keep * scale * x over n values in row-major order. The same call on the gradient is its backward.
+//
+// HBM-bound: each value is read once and written once, the mask is computed.
+#include "philox.cuh"
+
+namespace decik {
+namespace {
+
+template <typename X> __device__ __forceinline__ float load1(const X* p) { return Dt<X>::to_f(*p); }
+template <> __device__ __forceinline__ float load1<float>(const float* p) { return *p; }
+template <typename X> __device__ __forceinline__ void store1(X* p, float v) { *p = Dt<X>::from_f(v); }
+template <> __device__ __forceinline__ void store1<float>(float* p, float v) { *p = v; }
+
+// One thread per group of 8 values. Dropped values are 0 whatever x holds there (NaN included).
+template <typename X, typename O, bool RES>
+__global__ void __launch_bounds__(256)
+dropout_kernel(const X* x, const O* residual, O* out, int64_t n, uint32_t cut, float scale,
+               const int64_t* __restrict__ rng, int64_t stream_id) {
+  const philox::Key key = philox::make_key(rng, stream_id);
+  const int64_t groups = (n + 7) / 8;
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  for (int64_t g = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; g < groups; g += stride) {
+    const uint4 w = philox::words(key, static_cast<unsigned long long>(g));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int64_t i = 8 * g + j;
+      if (i >= n) break;
+      float v = philox::keep_lane(w, j, cut) ? load1(x + i) * scale : 0.f;
+      if constexpr (RES) v += load1(residual + i);
+      store1(out + i, v);
+    }
+  }
+}
+
+template <typename X, typename O>
+int launch(const void* x, const void* residual, void* out, int64_t n, double p, const int64_t* rng, int64_t stream_id,
+           cudaStream_t s) {
+  const uint32_t cut = philox::cut_of(p);
+  const float scale = philox::scale_of(cut);
+  const int64_t want = ((n + 7) / 8 + 255) / 256, cap = static_cast<int64_t>(sm_count()) * 16;
+  const int grid = static_cast<int>(want < cap ? want : cap);
+  if (residual != nullptr)
+    dropout_kernel<X, O, true><<<grid, 256, 0, s>>>(static_cast<const X*>(x), static_cast<const O*>(residual),
+                                                    static_cast<O*>(out), n, cut, scale, rng, stream_id);
+  else
+    dropout_kernel<X, O, false><<<grid, 256, 0, s>>>(static_cast<const X*>(x), nullptr, static_cast<O*>(out), n, cut,
+                                                     scale, rng, stream_id);
+  return check_launch("dropout");
+}
+
+template <typename X>
+int launch_x(int out_dtype, const void* x, const void* residual, void* out, int64_t n, double p, const int64_t* rng,
+             int64_t stream_id, cudaStream_t s) {
+  if (out_dtype == DECIK_F32) return launch<X, float>(x, residual, out, n, p, rng, stream_id, s);
+  if (out_dtype == DECIK_BF16) return launch<X, __nv_bfloat16>(x, residual, out, n, p, rng, stream_id, s);
+  return launch<X, __half>(x, residual, out, n, p, rng, stream_id, s);
+}
+
+bool valid_dtype(int d) { return d == DECIK_F16 || d == DECIK_BF16 || d == DECIK_F32; }
+
+}  // namespace
+}  // namespace decik
+
+extern "C" int decik_dropout(const void* x, int x_dtype, const void* residual, void* out, int out_dtype, int64_t n,
+                             double p, const int64_t* rng, int64_t stream_id, void* stream) {
+  using namespace decik;
+  if (n < 0) return set_error(DECIK_ERR_INVALID, "dropout: n=%lld", (long long)n);
+  if (!philox::valid_p(p)) return set_error(DECIK_ERR_INVALID, "dropout: p=%g is not in [0, 1]", p);
+  if (!valid_dtype(x_dtype) || !valid_dtype(out_dtype))
+    return set_error(DECIK_ERR_INVALID, "dropout: dtypes %d -> %d are not F16/BF16/F32", x_dtype, out_dtype);
+  if (n == 0) return DECIK_OK;
+  if (!x || !out || !rng) return set_error(DECIK_ERR_INVALID, "dropout: null pointer");
+  cudaStream_t s = as_stream(stream);
+  if (x_dtype == DECIK_F32) return launch_x<float>(out_dtype, x, residual, out, n, p, rng, stream_id, s);
+  if (x_dtype == DECIK_BF16) return launch_x<__nv_bfloat16>(out_dtype, x, residual, out, n, p, rng, stream_id, s);
+  return launch_x<__half>(out_dtype, x, residual, out, n, p, rng, stream_id, s);
+}

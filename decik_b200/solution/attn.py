@@ -41,6 +41,63 @@ class FusedQKRope(torch.autograd.Function):
         return dq, dq.clone(), dk, None, None, None, None
 
 
+def _rows16(t):
+    """t [A, B, D] as the head kernels read it: D contiguous, pointer and strides 16-byte aligned."""
+    ok = (t.stride(2) == 1 and t.data_ptr() % 16 == 0
+          and all(t.shape[i] == 1 or t.stride(i) % 8 == 0 for i in (0, 1)))
+    return t if ok else t.contiguous()
+
+
+class QKNormRope(torch.autograd.Function):
+    """RMSNorm of each query and key head and RoPE in one node, for models that norm their heads: q, k
+    [T, H, D] (q_lora, like q, is added first; may be None), norm weights [D], cos / sin fp32
+    [T, rotary_dim] -> q [1, Hq, T, D], k [1, Hk, T, D] as FusedQKRope gives them. Backward returns the
+    gradients of q, q_lora, k and both weights; it keeps only the inputs."""
+
+    @staticmethod
+    def forward(ctx, q, q_lora, k, q_weight, k_weight, eps, cos, sin):
+        q, k = _rows16(q), _rows16(k)
+        q_lora = None if q_lora is None else _rows16(q_lora)
+        out_q, out_k = ops.qk_norm_rope_fwd(q, k, q_weight, k_weight, eps, cos, sin, q_lora=q_lora)
+        ctx.save_for_backward(q, q_lora, k, q_weight, k_weight, cos, sin)
+        ctx.eps = eps
+        return out_q.unsqueeze(0), out_k.unsqueeze(0)
+
+    @staticmethod
+    def backward(ctx, grad_q, grad_k):
+        q, q_lora, k, wq, wk, cos, sin = ctx.saved_tensors
+        dq, dk, dwq, dwk = ops.qk_norm_rope_bwd(_rows16(grad_q[0]), _rows16(grad_k[0]), q, k, wq, wk, ctx.eps, cos,
+                                                sin, q_lora=q_lora)
+        return (dq, None if q_lora is None else dq.clone(), dk, dwq.to(wq.dtype), dwk.to(wk.dtype), None, None, None)
+
+
+class AxesRope(torch.autograd.Function):
+    """RoPE by positions of several axes (int64 / int32 [axes, T]; ``sections`` frequencies of each axis),
+    with the norms of QKNormRope when the weights are given (both, or both None). q, q_lora, k and
+    the results as there."""
+
+    @staticmethod
+    def forward(ctx, q, q_lora, k, positions, inv_freq, sections, interleaved=False, q_weight=None, k_weight=None,
+                eps=0.0):
+        q, k = _rows16(q), _rows16(k)
+        q_lora = None if q_lora is None else _rows16(q_lora)
+        out_q, out_k = ops.rope_axes_fwd(q, k, positions, inv_freq, sections, interleaved, q_weight, k_weight, eps,
+                                         q_lora=q_lora)
+        kept = (q, q_lora, k) if q_weight is not None else (None, None, None)  # a plain rotation needs no inputs
+        ctx.save_for_backward(*kept, q_weight, k_weight, positions, inv_freq)
+        ctx.meta = (tuple(sections), interleaved, eps, q_lora is not None)
+        return out_q.unsqueeze(0), out_k.unsqueeze(0)
+
+    @staticmethod
+    def backward(ctx, grad_q, grad_k):
+        q, q_lora, k, wq, wk, positions, inv_freq = ctx.saved_tensors
+        sections, interleaved, eps, lora = ctx.meta
+        got = ops.rope_axes_bwd(_rows16(grad_q[0]), _rows16(grad_k[0]), positions, inv_freq, sections, interleaved,
+                                q=q, k=k, q_weight=wq, k_weight=wk, eps=eps, q_lora=q_lora)
+        dwq, dwk = (None, None) if wq is None else (got[2].to(wq.dtype), got[3].to(wk.dtype))
+        return (got[0], got[0].clone() if lora else None, got[1], None, None, None, None, dwq, dwk, None)
+
+
 class FusedAttentionBlock(torch.autograd.Function):
     """x -> packed causal GQA attention output [T, Hq, D] in one autograd node, for q/v LoRA
     without dropout. The arithmetic of the reference's chain (solution/attn.py:395-416: three

@@ -1,0 +1,71 @@
+"""Dropout without stored masks: a counter-based generator on the device (csrc/philox.cuh).
+
+The reference draws LoRA dropout with ``torch.native_dropout`` on the padded batch and keeps the mask
+(solution/varlen.py:42-63, solution/attn.py:130-203), which stays the default here. The Functions
+below take a generator state instead, (seed, offset) as an int64 [2] tensor on the device; a mask is
+a function of the state, a stream number and the value's index, and the backward pass computes it
+again. Nothing is drawn from torch's generators.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from .. import ops
+
+
+class CounterRNG:
+    """The state of the generator on one device. ``take(n)`` returns the state for the next n streams
+    (numbers 0 .. n - 1) as a tensor of its own and advances; both are enqueued on the current stream,
+    so a captured step draws new masks at each replay. Ranks of a data-parallel job take different
+    seeds."""
+
+    def __init__(self, seed: int | None = None, device="cuda"):
+        seed = torch.initial_seed() if seed is None else int(seed)
+        seed = (seed + 2 ** 63) % 2 ** 64 - 2 ** 63  # as int64
+        self.state = torch.tensor([seed, 0], dtype=torch.int64, device=device)
+
+    def take(self, n: int = 1) -> torch.Tensor:
+        now = self.state.clone()
+        self.state[1] += n
+        return now
+
+
+class CounterDropout(torch.autograd.Function):
+    """dropout(x), or residual + dropout(x), with the mask of (rng, stream): ops.dropout. ``rng`` is kept
+    for the backward pass and must not be advanced in place before it (CounterRNG.take's are not)."""
+
+    @staticmethod
+    def forward(ctx, x, p, rng, stream=0, residual=None):
+        ctx.save_for_backward(rng)
+        ctx.meta = (p, stream, x.dtype, residual is not None)
+        return ops.dropout(x, p, rng, stream, residual=residual)
+
+    @staticmethod
+    def backward(ctx, grad):
+        (rng,) = ctx.saved_tensors
+        p, stream, dtype, residual = ctx.meta
+        return ops.dropout(grad, p, rng, stream, out_dtype=dtype), None, None, None, grad if residual else None
+
+
+class LoRADownDropout(torch.autograd.Function):
+    """The LoRA down projections of x [T, W] under dropout, u [T, branches * rank] =
+    scale_b (keep_b x16) A_b^T with a mask for each branch (ops.lora_down_dropout). ``a``: the branches'
+    lora_A weights [rank, W] (fp32, as peft keeps them), ``p`` the probability of each, ``dtype`` the
+    compute dtype. Keeps the 16-bit input only."""
+
+    @staticmethod
+    def forward(ctx, x, p, rng, stream, dtype, *a):
+        a16 = torch.cat(a).to(dtype)
+        x16, u = ops.lora_down_dropout(x if x.dtype == dtype else x.float(), a16, p, rng, stream)
+        ctx.save_for_backward(x16, a16, rng)
+        ctx.meta = (p, stream, x.dtype, [w.dtype for w in a])
+        return u
+
+    @staticmethod
+    def backward(ctx, du):
+        x16, a16, rng = ctx.saved_tensors
+        p, stream, x_dtype, a_dtypes = ctx.meta
+        dx, da = ops.lora_down_dropout_bwd(du.contiguous(), x16, a16, p, rng, stream)
+        parts = da.split(da.shape[0] // len(a_dtypes))
+        return (dx.to(x_dtype), None, None, None, None) + tuple(w.to(t) for w, t in zip(parts, a_dtypes))

@@ -452,6 +452,94 @@ DECIK_API int decik_mlp_down_grad(const void* grad, int64_t ldg, const void* w_d
                                   int64_t ldgu, void* dgu, int64_t lddgu, int64_t m, int hidden, int inter, int dtype,
                                   void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Dropout from a counter-based generator: no mask is stored, a backward pass computes it again.
+ * No counterpart in the reference, whose LoRA dropout draws a [batch, seq, width] mask and keeps it
+ * bit-packed (solution/attn.py:130-203, solution/varlen.py:42-63).
+ *
+ * The mask of (rng, stream_id) at index i of a row-major tensor: 16 bits of Philox4x32 with 7 rounds,
+ * key = seed, counter = (i / 8, offset + stream_id), lane i % 8 (the low half of a word first); the value
+ * is kept iff they are >= cut = floor(p 65536 + 1/2), and is then scaled by 65536 / (65536 - cut). So p
+ * counts in steps of 2^-16; p = 0 keeps everything, p = 1 nothing. A dropped value is 0, whatever x
+ * holds there (NaN and infinities included).
+ *   rng  int64 [2] on the device: seed, offset. It is read by the kernels, so a captured graph draws
+ *        anew when the caller advances the offset between replays; a backward pass needs the values
+ *        that the forward pass saw.
+ *
+ * decik_dropout: out = keep scale x, or with residual (out's type, may be NULL) residual + keep scale x,
+ * over n values; one rounding, to out's type. x, out: F16, BF16 or F32 each, of any alignment; out
+ * may be x or residual. The backward of the dropout is the same call on the gradient. */
+DECIK_API int decik_dropout(const void* x, int x_dtype, const void* residual, void* out, int out_dtype, int64_t n,
+                            double p, const int64_t* rng, int64_t stream_id, void* stream);
+
+/* The LoRA down projections of one input under such dropout, branch b (of n_branch, 1 or 2) with its own
+ * mask, that of stream_id + b over the [n_tok, width] input, and its own p:
+ *   x16 = dt(x),  u_b = dt(scale_b sum_k keep_b x16[t, k] A_b[r, k])     (fp32 sums)
+ *   x    [n_tok, width] F32 or dt (ldx);  a  dt [n_branch rank, width] (lda): the branches' lora_A
+ *   x16  dt [n_tok, width] (ldx16), may be NULL;  u  dt [n_tok, n_branch rank] (ldu)
+ * Replaces lora_A(dropout(x)) of the reference's LoRA branches (solution/attn.py:217-228) without its
+ * masks and masked copies. Backward, from du dt [n_tok, n_branch rank] (ld_du) and the forward's x16:
+ *   dx = addend + sum_b scale_b keep_b (du_b A_b)      fp32 [n_tok, width]
+ *   da_b = scale_b du_b^T (keep_b x16)                 fp32 [n_branch rank, width], contiguous
+ * addend fp32 (ld_add) may be NULL, or dx itself. The sums run in a fixed order: the same inputs give
+ * the same bits. workspace: decik_lora_down_dropout_bwd_workspace() bytes, 16-byte aligned.
+ * width % 8 == 0; rank % 8 == 0, the branches' ranks rounded up to 16 together <= 64; rows and
+ * pointers 16-byte aligned. */
+DECIK_API int decik_lora_down_dropout(const void* x, int x_dtype, int64_t ldx, const void* a, int64_t lda, void* x16,
+                                      int64_t ldx16, void* u, int64_t ldu, int64_t n_tok, int width, int rank,
+                                      int n_branch, double p0, double p1, const int64_t* rng, int64_t stream_id,
+                                      int dtype, void* stream);
+DECIK_API int64_t decik_lora_down_dropout_bwd_workspace(int64_t n_tok, int width, int rank, int n_branch);
+DECIK_API int decik_lora_down_dropout_bwd(const void* du, int64_t ld_du, const void* x16, int64_t ldx, const void* a,
+                                          int64_t lda, const float* addend, int64_t ld_add, float* dx, int64_t ld_dx,
+                                          float* da, int64_t n_tok, int width, int rank, int n_branch, double p0,
+                                          double p1, const int64_t* rng, int64_t stream_id, int dtype,
+                                          void* workspace, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * The norm of each query and key head with the position rotation in the same pass, and the rotation
+ * by positions of several axes. They stand beside decik_rope_fwd / _bwd for models with such heads; no
+ * counterpart in the reference. For the row x = q (+ q_lora) of one token and head, R = rotary_dim:
+ *   y = x rsqrt(mean(x^2) + eps) w   (y = x where the weights are NULL)
+ *   out[j] = y[j] cos[j] - y[j + R/2] sin[j],  out[j + R/2] = y[j + R/2] cos[j + R/2] + y[j] sin[j + R/2]
+ *   for j < R / 2, out[d] = y[d] for d >= R;   fp32 arithmetic, one rounding.
+ *   q, q_lora, k  [n_tok, heads, head_dim] views of dtype (F16 / BF16); q_lora.ptr may be NULL
+ *   q_weight, k_weight  [head_dim] of w_dtype (F32, F16, BF16)
+ *   q_out, k_out  views of the same shapes (head-major or token-major, by their strides)
+ * decik_qk_norm_rope_*: cos, sin fp32 [n_tok, rotary_dim], 16-byte aligned; both norm weights.
+ * decik_rope_axes_*: the angle of frequency j < R / 2 is positions[axis_of[j]][t] * inv_freq[j], reduced in
+ * 64 bits; positions int64 (pos_dtype 0) or int32 (1) [n_axes, n_tok] with rows ld_pos apart, inv_freq
+ * fp32 [R / 2] on the device, axis_of a HOST array of R / 2 bytes (each < n_axes <= 4), read during the
+ * call; the norm weights both given or both NULL.
+ * Backward, from grad_q / grad_k and the forward's inputs (q, q_lora, k are read only with norms):
+ *   dq, dk  views of dtype (dq is the gradient of q and of q_lora)
+ *   dq_weight, dk_weight  fp32 [head_dim], written whole (with norms), summed in a fixed order;
+ *   workspace: decik_qk_norm_rope_bwd_workspace() bytes, 16-byte aligned (with norms).
+ * head_dim and rotary_dim multiples of 16, rotary_dim <= head_dim <= 256; views 16-byte aligned. */
+DECIK_API int decik_qk_norm_rope_fwd(decik_tensor3 q, decik_tensor3 q_lora, decik_tensor3 k, const void* q_weight,
+                                     const void* k_weight, int w_dtype, float eps, const float* cos, const float* sin,
+                                     decik_tensor3_mut q_out, decik_tensor3_mut k_out, int64_t n_tok, int n_heads,
+                                     int n_kv, int head_dim, int rotary_dim, int dtype, void* stream);
+DECIK_API int64_t decik_qk_norm_rope_bwd_workspace(int head_dim);
+DECIK_API int decik_qk_norm_rope_bwd(decik_tensor3 grad_q, decik_tensor3 grad_k, decik_tensor3 q, decik_tensor3 q_lora,
+                                     decik_tensor3 k, const void* q_weight, const void* k_weight, int w_dtype,
+                                     float eps, const float* cos, const float* sin, decik_tensor3_mut dq,
+                                     decik_tensor3_mut dk, float* dq_weight, float* dk_weight, int64_t n_tok,
+                                     int n_heads, int n_kv, int head_dim, int rotary_dim, int dtype, void* workspace,
+                                     void* stream);
+DECIK_API int decik_rope_axes_fwd(decik_tensor3 q, decik_tensor3 q_lora, decik_tensor3 k, const void* q_weight,
+                                  const void* k_weight, int w_dtype, float eps, const void* positions, int pos_dtype,
+                                  int64_t ld_pos, int n_axes, const float* inv_freq, const uint8_t* axis_of,
+                                  decik_tensor3_mut q_out, decik_tensor3_mut k_out, int64_t n_tok, int n_heads,
+                                  int n_kv, int head_dim, int rotary_dim, int dtype, void* stream);
+DECIK_API int decik_rope_axes_bwd(decik_tensor3 grad_q, decik_tensor3 grad_k, decik_tensor3 q, decik_tensor3 q_lora,
+                                  decik_tensor3 k, const void* q_weight, const void* k_weight, int w_dtype, float eps,
+                                  const void* positions, int pos_dtype, int64_t ld_pos, int n_axes,
+                                  const float* inv_freq, const uint8_t* axis_of, decik_tensor3_mut dq,
+                                  decik_tensor3_mut dk, float* dq_weight, float* dk_weight, int64_t n_tok,
+                                  int n_heads, int n_kv, int head_dim, int rotary_dim, int dtype, void* workspace,
+                                  void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,205 @@
+"""The operators of the attention inputs without a GPU: the generator against published vectors, the
+oracles against each other and against differences, and the refusals of the C entry points (argument
+checks that fail before any CUDA call)."""
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from decik_b200 import _lib, ops
+from oracle import dropout as o_drop
+from oracle import head_rope as o_rope
+
+
+@pytest.mark.parametrize("counter,key,want", [
+    ((0, 0, 0, 0), (0, 0), "5f6fb709 0d893f64 4f121f81 4f730a48"),
+    ((0xFFFFFFFF,) * 4, (0xFFFFFFFF,) * 2, "5207ddc2 45165e59 4d8ee751 8c52f662"),
+    ((0x243F6A88, 0x85A308D3, 0x13198A2E, 0x03707344), (0xA4093822, 0x299F31D0),
+     "4dfccaba 190a87f0 c47362ba b6b5242a")])
+def test_philox_published_vectors(counter, key, want):
+    """The known answers of Philox4x32-7 that its authors publish with it."""
+    got = o_drop.philox(np.asarray([counter], dtype=np.uint64), key)[0]
+    assert " ".join(f"{int(v):08x}" for v in got) == want
+
+
+def test_masks_are_addressed_by_index_and_stream():
+    whole = o_drop.keep(4000, 0.3, 5, 2 ** 33 + 1, 3)
+    assert np.array_equal(whole[1600:], o_drop.keep(2400, 0.3, 5, 2 ** 33 + 1, 3, start=1600))
+    assert np.array_equal(whole, o_drop.keep(4000, 0.3, 5, 2 ** 33 + 4))       # offset + stream
+    other = o_drop.keep(4000, 0.3, 5, 2 ** 33 + 1, 4)
+    # two streams are independent: they agree with probability .7^2 + .3^2 = .58, sigma 0.0078
+    assert abs((whole == other).mean() - 0.58) < 5 * 0.0078
+    assert abs(whole.mean() - 0.7) < 5 * (0.21 / 4000) ** 0.5
+    assert o_drop.keep(64, 0.0, 1, 1).all() and not o_drop.keep(64, 1.0, 1, 1).any()
+
+
+@pytest.mark.parametrize("sections,interleaved,want", [
+    ((3, 2, 1), False, [0, 0, 0, 1, 1, 2]), ((3, 2, 1), True, [0, 1, 2, 0, 1, 0]), ((0, 4), True, [1, 1, 1, 1]),
+    ((24, 20, 20), True, [0, 1, 2] * 20 + [0] * 4)])
+def test_axis_of(sections, interleaved, want):
+    assert list(ops.rope_axis_of(sections, interleaved)) == want == list(o_rope.axis_of(sections, interleaved))
+
+
+@pytest.mark.parametrize("sections", [(), (1, 1, 1, 1, 1), (4, -1), (2.5, 1)])
+def test_axis_of_refusals(sections):
+    with pytest.raises(RuntimeError, match="sections"):
+        ops.rope_axis_of(sections)
+
+
+@pytest.mark.parametrize("normed", [True, False])
+def test_head_rope_oracle_gradient(normed):
+    """The backward formulas against central differences of the forward, in 64 bits."""
+    rng = np.random.default_rng(0)
+    T, H, D, R = 3, 2, 32, 16
+    x, g = rng.standard_normal((T, H, D)), rng.standard_normal((T, H, D))
+    w = 1 + 0.3 * rng.standard_normal(D) if normed else None
+    cos, sin = rng.standard_normal((T, R)), rng.standard_normal((T, R))  # any tables, not only rotations
+    loss = lambda x, w: (o_rope.forward(x, w, 0.1, cos, sin)[0] * g).sum()
+    dx, _, dw, _ = o_rope.backward(g, x, w, 0.1, cos, sin)
+    h = 1e-5
+    for i in [(0, 0, 0), (1, 1, 7), (2, 0, 9), (2, 1, 20), (0, 1, 31)]:
+        e = np.zeros_like(x)
+        e[i] = h
+        assert abs((loss(x + e, w) - loss(x - e, w)) / (2 * h) - dx[i]) < 1e-8 * max(1, abs(dx[i])) + 1e-8
+        if normed:
+            e = np.zeros(D)
+            e[i[2]] = h
+            assert abs((loss(x, w + e) - loss(x, w - e)) / (2 * h) - dw[i[2]]) < 1e-8 * max(1, abs(dw[i[2]])) + 1e-8
+
+
+def test_lora_oracle_gradient():
+    """dx and dA of the dropped-out down projections against differences (the mask is a constant)."""
+    rng = np.random.default_rng(1)
+    T, W, r, p = 3, 16, 8, (0.3, 0.6)
+    x, a, du = rng.standard_normal((T, W)), rng.standard_normal((2 * r, W)), rng.standard_normal((T, 2 * r))
+    loss = lambda x, a: (o_drop.lora_down(x, a, p, 7, 9, 2)[0] * du).sum()
+    dx, da, _, _ = o_drop.lora_down_bwd(du, x, a, p, 7, 9, 2)
+    h = 1e-5
+    for t, k, j in [(0, 0, 0), (1, 5, 3), (2, 15, 15), (1, 9, 8)]:
+        e = np.zeros_like(x)
+        e[t, k] = h
+        assert abs((loss(x + e, a) - loss(x - e, a)) / (2 * h) - dx[t, k]) < 1e-7
+        e = np.zeros_like(a)
+        e[j, k] = h
+        assert abs((loss(x, a + e) - loss(x, a - e)) / (2 * h) - da[j, k]) < 1e-7
+
+
+# ------------------------------------------------------------------------------------ refusals
+P = ctypes.c_void_p(256)   # never dereferenced: the checks fail before any CUDA call
+ODD = ctypes.c_void_p(260)
+T3 = _lib.Tensor3
+NONE3 = T3(None, 0, 0)
+
+
+def _v(ts=256, hs=128, ptr=256):
+    return T3(ptr, ts, hs)
+
+
+def _refused(rc, text, code=1):
+    assert rc == code, rc
+    assert text in _lib.lib().decik_last_error()
+
+
+@pytest.mark.parametrize("p", [-0.1, 1.5, float("nan")])
+def test_dropout_refuses_p(p):
+    lib = _lib.lib()
+    _refused(lib.decik_dropout(P, 1, None, P, 1, 8, p, P, 0, None), b"not in [0, 1]")
+    _refused(lib.decik_lora_down_dropout(P, 2, 64, P, 64, P, 64, P, 32, 4, 64, 16, 2, 0.1, p, P, 0, 1, None),
+             b"not in [0, 1]")
+
+
+def test_dropout_refusals():
+    lib = _lib.lib()
+    _refused(lib.decik_dropout(P, 3, None, P, 1, 8, 0.1, P, 0, None), b"dtypes")
+    _refused(lib.decik_dropout(P, 1, None, P, 1, -1, 0.1, P, 0, None), b"n=-1")
+    _refused(lib.decik_dropout(P, 1, None, P, 1, 8, 0.1, None, 0, None), b"null pointer")
+    assert lib.decik_dropout(None, 1, None, None, 1, 0, 0.1, None, 0, None) == 0
+
+
+def test_lora_refusals():
+    lib = _lib.lib()
+    fwd = lambda x=P, xd=2, ldx=64, ldu=32, n=4, w=64, r=16, nb=2, dt=1: lib.decik_lora_down_dropout(
+        x, xd, ldx, P, 64, P, 64, P, ldu, n, w, r, nb, 0.1, 0.1, P, 0, dt, None)
+    _refused(fwd(w=60), b"width 60")
+    _refused(fwd(n=-1), b"T=-1")
+    _refused(fwd(r=12), b"rank 12", 3)
+    _refused(fwd(r=40), b"rank 40", 3)      # 2 branches of 48 rows
+    _refused(fwd(nb=3), b"3 branches", 3)
+    _refused(fwd(dt=2), b"dtype 2")
+    _refused(fwd(xd=0), b"x of dtype 0")
+    _refused(fwd(ldx=56), b"strides shorter")
+    _refused(fwd(ldu=24), b"strides shorter")
+    _refused(fwd(x=ODD), b"alignment")
+    _refused(fwd(ldx=66), b"alignment")
+    assert fwd(n=0) == 0
+    bwd = lambda du=P, ws=P, da=P, ldx=64, ldd=64, n=4: lib.decik_lora_down_dropout_bwd(
+        du, 32, P, ldx, P, 64, None, 0, P, ldd, da, n, 64, 16, 2, 0.1, 0.1, P, 0, 1, ws, None)
+    _refused(bwd(du=None), b"null pointer")
+    _refused(bwd(ws=None), b"null pointer")
+    _refused(bwd(da=None), b"da NULL")
+    _refused(bwd(ldx=60), b"strides shorter")
+    _refused(bwd(ldd=66), b"alignment")
+    _refused(bwd(n=1 << 31), b"T=")
+    assert lib.decik_lora_down_dropout_bwd_workspace(0, 64, 16, 2) == 0
+    assert lib.decik_lora_down_dropout_bwd_workspace(1000, 64, 16, 2) >= 4 * 64 * 32
+
+
+def test_norm_rope_refusals():
+    lib = _lib.lib()
+
+    def fwd(q=_v(), k=_v(), wq=P, wk=P, wd=2, eps=1e-6, cos=P, n=4, D=128, R=128, dt=1):
+        return lib.decik_qk_norm_rope_fwd(q, NONE3, k, wq, wk, wd, eps, cos, P, _v(), _v(), n, 2, 1, D, R, dt, None)
+
+    _refused(fwd(D=120), b"head_dim 120")
+    _refused(fwd(D=272), b"head_dim 272")
+    _refused(fwd(R=144), b"rotary_dim 144")
+    _refused(fwd(R=24), b"rotary_dim 24")
+    _refused(fwd(R=0), b"rotary_dim 0")
+    _refused(fwd(wq=None), b"NULL norm weight")
+    _refused(fwd(wd=5), b"norm weights of dtype 5")
+    _refused(fwd(eps=-1.0), b"eps")
+    _refused(fwd(eps=float("nan")), b"eps")
+    _refused(fwd(cos=None), b"cos / sin")
+    _refused(fwd(cos=ODD), b"cos / sin")
+    _refused(fwd(q=_v(ptr=264)), b"aligned")
+    _refused(fwd(k=_v(ts=252)), b"aligned")
+    _refused(fwd(dt=2), b"dtype 2")
+    assert fwd(n=0) == 0
+    bwd = lambda ws=P, dw=P, gq=_v(): lib.decik_qk_norm_rope_bwd(
+        gq, _v(), _v(), NONE3, _v(), P, P, 2, 1e-6, P, P, _v(), _v(), dw, P, 4, 2, 1, 128, 128, 1, ws, None)
+    _refused(bwd(ws=None), b"workspace")
+    _refused(bwd(ws=ODD), b"workspace")
+    _refused(bwd(dw=None), b"dq_weight")
+    _refused(bwd(gq=NONE3), b"aligned")
+
+
+def test_axes_refusals():
+    lib = _lib.lib()
+
+    def fwd(pos=P, pd=0, ld=4, axes=3, inv=P, amap=bytes([0, 1, 2, 0] * 16), wq=None, wk=None, n=4, R=128):
+        return lib.decik_rope_axes_fwd(_v(), NONE3, _v(), wq, wk, 2, 1e-6, pos, pd, ld, axes, inv, amap, _v(), _v(), n,
+                                       2, 1, 128, R, 1, None)
+
+    _refused(fwd(axes=5), b"5 axes")
+    _refused(fwd(axes=0), b"0 axes")
+    _refused(fwd(pd=2), b"position dtype 2")
+    _refused(fwd(pos=None), b"null pointer")
+    _refused(fwd(inv=None), b"null pointer")
+    _refused(fwd(amap=None), b"null pointer")
+    _refused(fwd(ld=3), b"rows of positions")
+    _refused(fwd(amap=bytes([0, 1, 3, 0] * 16)), b"frequency 2 has axis 3 of 3")
+    _refused(fwd(wq=P), b"for neither")
+    _refused(fwd(R=8), b"rotary_dim 8")
+    assert fwd(n=0) == 0
+
+
+def test_ops_refuse_cpu_tensors():
+    q, k = torch.zeros(4, 2, 64, dtype=torch.bfloat16), torch.zeros(4, 1, 64, dtype=torch.bfloat16)
+    w, cs, rng = torch.ones(64), torch.ones(4, 64), torch.zeros(2, dtype=torch.int64)
+    for call in (lambda: ops.qk_norm_rope_fwd(q, k, w, w, 1e-6, cs, cs), lambda: ops.dropout(cs, 0.1, rng),
+                 lambda: ops.rope_axes_fwd(q, k, torch.zeros(1, 4, dtype=torch.int64), torch.ones(32), (32,)),
+                 lambda: ops.lora_down_dropout(cs, q[:, 0], 0.1, rng)):
+        with pytest.raises(RuntimeError, match="one CUDA device"):
+            call()
