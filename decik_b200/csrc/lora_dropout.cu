@@ -5,6 +5,7 @@
 //   backward  dx = addend + sum_b s_b keep_b o (du_b A_b),  dA_b = s_b du_b^T (keep_b o x16)
 // The index of x[t, k] is t * width + k (width % 8 == 0: a group of 8 stays in one row).
 #include "philox.cuh"
+#include "ptx.cuh"
 
 namespace decik {
 namespace loradrop {
@@ -17,101 +18,302 @@ struct Drop {  // per branch
   float scale[2];
 };
 
-template <typename X> __device__ __forceinline__ float load1(const X* p) { return Dt<X>::to_f(*p); }
-template <> __device__ __forceinline__ float load1<float>(const float* p) { return *p; }
-
-// One CTA per row: the masked 16-bit row of each branch in turn, then one warp per row of A.
-template <typename X, typename T>
-__global__ void __launch_bounds__(256)
-down_kernel(const X* x, int64_t ldx, const T* __restrict__ a, int64_t lda, T* x16, int64_t ldx16, T* __restrict__ u,
-            int64_t ldu, int width, int rank, int branches, Drop d, const int64_t* __restrict__ rng,
-            int64_t stream_id) {
-  const int64_t t = blockIdx.x;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int col = warp; col < rank * branches; col += 8) {
-    const int b = col / rank;
-    const philox::Key key = philox::make_key(rng, stream_id + b);
-    float acc = 0.f;
-    for (int g = lane; g < width / 8; g += 32) {
-      const uint4 w = philox::words(key, static_cast<unsigned long long>(t) * (width / 8) + g);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int k = 8 * g + j;
-        if (philox::keep_lane(w, j, d.cut[b]))
-          acc += Dt<T>::to_f(Dt<T>::from_f(load1(x + t * ldx + k))) * Dt<T>::to_f(a[col * lda + k]);
-      }
-    }
-    for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-    if (lane == 0) u[t * ldu + col] = Dt<T>::from_f(acc * d.scale[b]);
-  }
-  if (x16 != nullptr)
-    for (int k = threadIdx.x; k < width; k += blockDim.x) x16[t * ldx16 + k] = Dt<T>::from_f(load1(x + t * ldx + k));
+// the kept values of a 16-bit pair v under the two lanes of one word of the generator
+__device__ __forceinline__ uint32_t mask_pair(uint32_t w, uint32_t v, uint32_t cut) {
+  const uint32_t m = ((w & 0xFFFFu) >= cut ? 0x0000FFFFu : 0u) | ((w >> 16) >= cut ? 0xFFFF0000u : 0u);
+  return v & m;
+}
+__device__ __forceinline__ void mask8(const uint4& w, const uint4& v, uint32_t cut, uint32_t (&m)[4]) {
+  m[0] = mask_pair(w.x, v.x, cut);
+  m[1] = mask_pair(w.y, v.y, cut);
+  m[2] = mask_pair(w.z, v.z, cut);
+  m[3] = mask_pair(w.w, v.w, cut);
 }
 
-// One thread per group of 8 columns of one token.
-template <typename T>
-__global__ void __launch_bounds__(256)
-dx_kernel(const T* __restrict__ du, int64_t ld_du, const T* __restrict__ a, int64_t lda, const float* addend,
-          int64_t ld_add, float* dx, int64_t ld_dx, int64_t n_tok, int width, int rank, int branches, Drop d,
-          const int64_t* __restrict__ rng, int64_t stream_id) {
-  const int64_t gw = width / 8, total = n_tok * gw, stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += stride) {
-    const int64_t t = i / gw;
-    const int k = 8 * static_cast<int>(i % gw);
-    float out[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) out[j] = addend != nullptr ? addend[t * ld_add + k + j] : 0.f;
-    for (int b = 0; b < branches; ++b) {
-      const uint4 w = philox::words(philox::make_key(rng, stream_id + b), static_cast<unsigned long long>(i));
-      float acc[8] = {};
-      for (int r = b * rank; r < (b + 1) * rank; ++r) {
-        const float g = Dt<T>::to_f(du[t * ld_du + r]);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) acc[j] += g * Dt<T>::to_f(a[r * lda + k + j]);
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) out[j] += philox::keep_lane(w, j, d.cut[b]) ? d.scale[b] * acc[j] : 0.f;
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) dx[t * ld_dx + k + j] = out[j];
+// 8 consecutive values of x as 16-bit pairs
+template <typename T, typename X>
+__device__ __forceinline__ uint4 load8(const X* p) {
+  if constexpr (sizeof(X) == 2) {
+    return ldg16(p);
+  } else {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    const float f[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    return pack8<T>(f);
   }
 }
 
-constexpr int kChunk = 512;  // tokens of one partial sum of dA
+// transpose of an 8 x 8 matrix of 16-bit values held by a warp (lane 4 i + c: row i, columns 2 c, 2 c + 1)
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
 
-// Partial dA of one token chunk (blockIdx.y): one thread per (row of A, group of 8 columns).
-template <typename T>
-__global__ void __launch_bounds__(256)
-da_kernel(const T* __restrict__ du, int64_t ld_du, const T* __restrict__ x16, int64_t ldx, float* __restrict__ part,
-          int64_t n_tok, int width, int rank, int branches, Drop d, const int64_t* __restrict__ rng,
-          int64_t stream_id) {
-  const int gw = width / 8, i = blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= gw * rank * branches) return;
-  const int r = i / gw, g = i % gw, b = r / rank;
-  const philox::Key key = philox::make_key(rng, stream_id + b);
-  const int64_t t0 = static_cast<int64_t>(blockIdx.y) * kChunk, t1 = t0 + kChunk < n_tok ? t0 + kChunk : n_tok;
-  float acc[8] = {};
-  for (int64_t t = t0; t < t1; ++t) {
-    const uint4 w = philox::words(key, static_cast<unsigned long long>(t) * gw + g);
-    const float du_r = Dt<T>::to_f(du[t * ld_du + r]);
+// ------------------------------------------------------------------------------------------------
+// forward
+// ------------------------------------------------------------------------------------------------
+// A CTA takes 16 MT rows; its 8 warps share out the width in blocks of 32 columns and their partial
+// sums meet in shared memory. In a block, lane 4 g + c holds the 8 columns from 8 c of rows g and g + 8
+// (of each 16): 32 bytes of x in one go, one call of the generator per row and branch, and, because
+// the order of a sum's terms is free, an operand fragment of mma.sync m16n8k16 without any exchange:
+// the instruction's columns 2 c, 2 c + 1 and 2 c + 8, 2 c + 9 of step s are the lane's pairs 2 s and
+// 2 s + 1. lora_A's rows, read the same way (16 bytes of row g), are the other operand.
+constexpr int kWarps = 8;
+
+template <typename X, typename T, int NB, int NTB, int MT>
+__global__ void __launch_bounds__(32 * kWarps, NB * NTB <= 4 ? 2 : 1)
+down_kernel(const X* __restrict__ x, int64_t ldx, const T* __restrict__ a, int64_t lda, T* __restrict__ x16,
+            int64_t ldx16, T* __restrict__ u, int64_t ldu, int64_t n_tok, int width, int rank, Drop d,
+            const int64_t* __restrict__ rng, int64_t stream_id) {
+  constexpr int NT = NB * NTB;            // n8 tiles of u's columns
+  constexpr int LD = 8 * NT + 4;
+  __shared__ float red[kWarps][16][LD];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * (16 * MT);
+  philox::Key key[NB];
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (philox::keep_lane(w, j, d.cut[b])) acc[j] += du_r * Dt<T>::to_f(x16[t * ldx + 8 * g + j]);
+  for (int b = 0; b < NB; ++b) key[b] = philox::make_key(rng, stream_id + b);
+  float acc[MT][NT][4];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[m][n][e] = 0.f;
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+  for (int k = 32 * warp + 8 * c; k - 8 * c < width; k += 32 * kWarps) {
+    const bool in = k < width;
+    uint4 xv[MT][2];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int64_t t = t0 + 16 * m + 8 * h + g;
+        xv[m][h] = in && t < n_tok ? load8<T>(x + t * ldx + k) : zero;
+      }
+    uint4 av[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int r = 8 * (n % NTB);
+      av[n] = in && r < rank ? ldg16(a + static_cast<int64_t>(n / NTB * rank + r + g) * lda + k) : zero;
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int64_t t = t0 + 16 * m + 8 * h + g;
+        if (x16 != nullptr && in && t < n_tok) stg16(x16 + t * ldx16 + k, xv[m][h]);
+      }
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        uint32_t lo[4], hi[4];
+        const unsigned long long group = static_cast<unsigned long long>(t0 + 16 * m + g) * (width / 8) + k / 8;
+        mask8(philox::words(key[b], group), xv[m][0], d.cut[b], lo);
+        mask8(philox::words(key[b], group + static_cast<unsigned long long>(width)), xv[m][1], d.cut[b], hi);
+        const uint32_t f0[4] = {lo[0], hi[0], lo[1], hi[1]}, f1[4] = {lo[2], hi[2], lo[3], hi[3]};
+#pragma unroll
+        for (int n = b * NTB; n < (b + 1) * NTB; ++n) {
+          ptx::mma16816<T>(acc[m][n], f0, av[n].x, av[n].y);
+          ptx::mma16816<T>(acc[m][n], f1, av[n].z, av[n].w);
+        }
+      }
+    }
   }
-  float* p = part + (static_cast<int64_t>(blockIdx.y) * rank * branches + r) * width + 8 * g;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) p[j] = acc[j];
+  for (int m = 0; m < MT; ++m) {
+    if (m > 0) __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      *reinterpret_cast<float2*>(&red[warp][g][8 * n + 2 * c]) = make_float2(acc[m][n][0], acc[m][n][1]);
+      *reinterpret_cast<float2*>(&red[warp][g + 8][8 * n + 2 * c]) = make_float2(acc[m][n][2], acc[m][n][3]);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 16 * 4 * NT; i += 32 * kWarps) {  // a pair of u's columns
+      const int row = i / (4 * NT), col = 2 * (i % (4 * NT)), b = col / (8 * NTB), r = col % (8 * NTB);
+      const int64_t t = t0 + 16 * m + row;
+      if (t >= n_tok || r >= rank) continue;
+      float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float2 v = *reinterpret_cast<const float2*>(&red[w][row][col]);
+        s.x += v.x;
+        s.y += v.y;
+      }
+      const float scale = NB == 2 && b == 1 ? d.scale[1] : d.scale[0];
+      *reinterpret_cast<uint32_t*>(u + t * ldu + b * rank + r) = Dt<T>::pack2(s.x * scale, s.y * scale);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// backward
+// ------------------------------------------------------------------------------------------------
+// One pass gives dx and the partial dA: both need the same masks, and x16, the addend and dx are read
+// or written once. A warp owns 32 columns and walks over its chunk of tokens in tiles of 16, with dA's
+// 32 columns in its accumulators. Lane 4 g + c holds the 8 columns from 8 c of tokens g and g + 8, as in
+// the forward. With the columns of an n8 tile j numbered n <-> 8 (n / 2) + 2 j + n % 2, both products fit
+// these registers:
+//   P = du A (m = token, k = rank): the accumulators of tiles 0..3 are the lane's own 8 columns, so mask,
+//       scale and addend are applied in place and dx leaves in 16-byte pieces;
+//   dA += du^T (keep x) (m = rank, k = token): the masked pair j of the lanes, as an 8 x 8 matrix
+//       (token, column), transposed by movmatrix is the operand fragment of tile j.
+template <typename T, int NB, int KR>
+__global__ void __launch_bounds__(128, NB * KR <= 2 ? 4 : 2)
+bwd_kernel(const T* __restrict__ du, int64_t ld_du, const T* __restrict__ x16, int64_t ldx, const T* __restrict__ a,
+           int64_t lda, const float* addend, int64_t ld_add, float* dx, int64_t ld_dx, float* __restrict__ part,
+           int64_t n_tok, int width, int rank, int chunk, int col_blocks, int n_units, Drop d,
+           const int64_t* __restrict__ rng, int64_t stream_id) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int unit = blockIdx.x * 4 + (threadIdx.x >> 5);  // (token chunk, block of 32 columns)
+  if (unit >= n_units) return;
+  const int cb = unit % col_blocks;
+  const int64_t first = static_cast<int64_t>(unit / col_blocks) * chunk;
+  const int64_t last = first + chunk < n_tok ? first + chunk : n_tok;
+  const int k = 32 * cb + 8 * c;
+  const bool in = k < width;
+  philox::Key key[NB];
+  uint32_t af[NB][KR][4][2];   // A as P's operand: rows (rank) 2 c, 2 c + 1 (+ 8) of column n = g of tile j
+  float acc[NB][KR][4][4];     // dA
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    key[b] = philox::make_key(rng, stream_id + b);
+#pragma unroll
+    for (int r = 0; r < KR; ++r)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int col = 32 * cb + 8 * (g >> 1) + 2 * j + (g & 1);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int row = 16 * r + 8 * h + 2 * c;
+          uint32_t v = 0u;
+          if (col < width && row < rank) {
+            const uint16_t* p = reinterpret_cast<const uint16_t*>(a + static_cast<int64_t>(b * rank + row) * lda + col);
+            v = static_cast<uint32_t>(p[0]) | static_cast<uint32_t>(p[lda]) << 16;
+          }
+          af[b][r][j][h] = v;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[b][r][j][e] = 0.f;
+      }
+  }
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+  for (int64_t t0 = first; t0 < last; t0 += 16) {
+    const int64_t t[2] = {t0 + g, t0 + g + 8};
+    const bool ok[2] = {t[0] < last, t[1] < last};
+    uint4 xv[2];
+    float out[2][8];
+    uint32_t df[NB][KR][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      xv[h] = ok[h] && in ? ldg16(x16 + t[h] * ldx + k) : zero;
+      float4 lo = make_float4(0.f, 0.f, 0.f, 0.f), hi = lo;
+      if (addend != nullptr && ok[h] && in) {
+        lo = *reinterpret_cast<const float4*>(addend + t[h] * ld_add + k);
+        hi = *reinterpret_cast<const float4*>(addend + t[h] * ld_add + k + 4);
+      }
+      out[h][0] = lo.x, out[h][1] = lo.y, out[h][2] = lo.z, out[h][3] = lo.w;
+      out[h][4] = hi.x, out[h][5] = hi.y, out[h][6] = hi.z, out[h][7] = hi.w;
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < KR; ++r)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {  // (tokens g | g + 8, ranks 2 c .. | 2 c + 8 ..)
+          const int h = q & 1, row = 16 * r + 8 * (q >> 1) + 2 * c;
+          df[b][r][q] = ok[h] && row < rank
+                            ? __ldg(reinterpret_cast<const unsigned int*>(du + t[h] * ld_du + b * rank + row)) : 0u;
+        }
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      uint32_t m[2][4];
+      float p[4][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) p[j][e] = 0.f;
+#pragma unroll
+        for (int r = 0; r < KR; ++r) ptx::mma16816<T>(p[j], df[b][r], af[b][r][j][0], af[b][r][j][1]);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint4 w = philox::words(key[b], static_cast<unsigned long long>(t[h]) * (width / 8) + k / 8);
+        mask8(w, xv[h], d.cut[b], m[h]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (philox::keep_lane(w, i, d.cut[b])) out[h][i] += d.scale[b] * p[i >> 1][2 * h + (i & 1)];
+      }
+      uint32_t bf[4][2];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) bf[j][h] = transpose8x8(m[h][j]);
+#pragma unroll
+      for (int r = 0; r < KR; ++r) {
+        const uint32_t dt[4] = {transpose8x8(df[b][r][0]), transpose8x8(df[b][r][2]), transpose8x8(df[b][r][1]),
+                                transpose8x8(df[b][r][3])};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ptx::mma16816<T>(acc[b][r][j], dt, bf[j][0], bf[j][1]);
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (ok[h] && in) {
+        float4* o = reinterpret_cast<float4*>(dx + t[h] * ld_dx + k);
+        o[0] = make_float4(out[h][0], out[h][1], out[h][2], out[h][3]);
+        o[1] = make_float4(out[h][4], out[h][5], out[h][6], out[h][7]);
+      }
+  }
+  if (!in) return;
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int r = 0; r < KR; ++r)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int row = 16 * r + 8 * h + g;
+        if (row >= rank) continue;
+        float4* o = reinterpret_cast<float4*>(
+            part + (static_cast<int64_t>(unit / col_blocks) * NB * rank + b * rank + row) * width + k);
+        o[0] = make_float4(acc[b][r][0][2 * h], acc[b][r][0][2 * h + 1], acc[b][r][1][2 * h], acc[b][r][1][2 * h + 1]);
+        o[1] = make_float4(acc[b][r][2][2 * h], acc[b][r][2][2 * h + 1], acc[b][r][3][2 * h], acc[b][r][3][2 * h + 1]);
+      }
 }
 
 // dA = scale * the sum of the chunks' partials, in chunk order (no atomics: the same bits every time)
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(128)
 da_sum_kernel(const float* __restrict__ part, float* __restrict__ da, int n_chunks, int width, int rank, int branches,
               Drop d) {
-  const int n = width * rank * branches, i = blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= n) return;
-  float acc = 0.f;
-  for (int c = 0; c < n_chunks; ++c) acc += part[static_cast<int64_t>(c) * n + i];
-  da[i] = d.scale[i / width / rank] * acc;
+  const int n4 = width / 4 * rank * branches, i = blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= n4) return;
+  const float4* p = reinterpret_cast<const float4*>(part) + i;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int c = 0; c < n_chunks; ++c) {
+    const float4 v = __ldg(p + static_cast<int64_t>(c) * n4);
+    s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+  }
+  const float scale = i / (width / 4) / rank == 1 ? d.scale[1] : d.scale[0];
+  reinterpret_cast<float4*>(da)[i] = make_float4(scale * s.x, scale * s.y, scale * s.z, scale * s.w);
+}
+
+// The token chunks of a backward pass: enough (chunk, 32 columns) units to give every SM 16 warps, at
+// most 1024 tokens each (dA's accumulators on the tensor cores truncate: a chain of at most 64 of
+// their sums, then fp32 additions), at least one tile of 16.
+struct Split {
+  int chunk, n_chunks, col_blocks;
+};
+Split split_of(int64_t n_tok, int width) {
+  Split s;
+  s.col_blocks = (width + 31) / 32;
+  const int64_t tiles = (n_tok + 15) / 16;
+  int64_t want = (static_cast<int64_t>(sm_count()) * 16 + s.col_blocks - 1) / s.col_blocks;
+  const int64_t least = (n_tok + 1023) / 1024;
+  if (want < least) want = least;
+  if (want > tiles) want = tiles;
+  s.chunk = static_cast<int>((tiles + want - 1) / want * 16);
+  s.n_chunks = static_cast<int>((n_tok + s.chunk - 1) / s.chunk);
+  return s;
 }
 
 int check_sizes(const char* what, int64_t n_tok, int width, int rank, int branches, double p0, double p1, int dtype) {
@@ -136,6 +338,41 @@ Drop make_drop(double p0, double p1) {
   return d;
 }
 
+struct DownArgs {
+  const void* x;
+  int64_t ldx;
+  const void* a;
+  int64_t lda;
+  void* x16;
+  int64_t ldx16;
+  void* u;
+  int64_t ldu, n_tok;
+  int width, rank;
+  Drop d;
+  const int64_t* rng;
+  int64_t stream_id;
+  cudaStream_t s;
+};
+
+template <typename X, typename T, int NB, int NTB>
+int launch_down_t(const DownArgs& p) {
+  auto go = [&](auto kernel, int rows) {
+    kernel<<<static_cast<unsigned>((p.n_tok + rows - 1) / rows), 32 * kWarps, 0, p.s>>>(
+        static_cast<const X*>(p.x), p.ldx, static_cast<const T*>(p.a), p.lda, static_cast<T*>(p.x16), p.ldx16,
+        static_cast<T*>(p.u), p.ldu, p.n_tok, p.width, p.rank, p.d, p.rng, p.stream_id);
+  };
+  if (p.n_tok <= 32 * static_cast<int64_t>(sm_count())) go(down_kernel<X, T, NB, NTB, 1>, 16);
+  else go(down_kernel<X, T, NB, NTB, 2>, 32);
+  return check_launch("lora_down_dropout");
+}
+
+template <typename X, typename T>
+int launch_down(const DownArgs& p, int branches) {
+  if (branches == 2) return p.rank <= 16 ? launch_down_t<X, T, 2, 2>(p) : launch_down_t<X, T, 2, 4>(p);
+  if (p.rank <= 16) return launch_down_t<X, T, 1, 2>(p);
+  return p.rank <= 32 ? launch_down_t<X, T, 1, 4>(p) : launch_down_t<X, T, 1, 8>(p);
+}
+
 }  // namespace
 }  // namespace loradrop
 }  // namespace decik
@@ -157,25 +394,17 @@ extern "C" int decik_lora_down_dropout(const void* x, int x_dtype, int64_t ldx, 
   if (ldx % xe || lda % 8 || (x16 && ldx16 % 8) || ldu % 8 || !aligned16(x) || !aligned16(a) ||
       (x16 && !aligned16(x16)) || !aligned16(u))
     return set_error(DECIK_ERR_INVALID, "lora_down_dropout: rows and pointers need 16-byte alignment");
-  const Drop d = make_drop(p0, p1);
-  cudaStream_t s = as_stream(stream);
+  const DownArgs p{x, ldx, a, lda, x16, ldx16, u, ldu, n_tok, width, rank, make_drop(p0, p1), rng, stream_id,
+                   as_stream(stream)};
   return DECIK_DISPATCH_16(dtype, [&] {
-    if (x_dtype == DECIK_F32)
-      down_kernel<float, T><<<static_cast<unsigned>(n_tok), 256, 0, s>>>(
-          static_cast<const float*>(x), ldx, static_cast<const T*>(a), lda, static_cast<T*>(x16), ldx16,
-          static_cast<T*>(u), ldu, width, rank, n_branch, d, rng, stream_id);
-    else
-      down_kernel<T, T><<<static_cast<unsigned>(n_tok), 256, 0, s>>>(
-          static_cast<const T*>(x), ldx, static_cast<const T*>(a), lda, static_cast<T*>(x16), ldx16,
-          static_cast<T*>(u), ldu, width, rank, n_branch, d, rng, stream_id);
-    return check_launch("lora_down_dropout");
+    return x_dtype == DECIK_F32 ? launch_down<float, T>(p, n_branch) : launch_down<T, T>(p, n_branch);
   });
 }
 
 extern "C" int64_t decik_lora_down_dropout_bwd_workspace(int64_t n_tok, int width, int rank, int n_branch) {
   using namespace decik::loradrop;
   if (n_tok <= 0 || width <= 0 || rank <= 0 || n_branch <= 0) return 0;
-  return (n_tok + kChunk - 1) / kChunk * rank * n_branch * width * static_cast<int64_t>(sizeof(float));
+  return split_of(n_tok, width).n_chunks * static_cast<int64_t>(sizeof(float)) * rank * n_branch * width;
 }
 
 extern "C" int decik_lora_down_dropout_bwd(const void* du, int64_t ld_du, const void* x16, int64_t ldx, const void* a,
@@ -200,19 +429,20 @@ extern "C" int decik_lora_down_dropout_bwd(const void* du, int64_t ld_du, const 
       !aligned16(a) || !aligned16(dx) || (addend && !aligned16(addend)) || !aligned16(workspace))
     return set_error(DECIK_ERR_INVALID, "lora_down_dropout_bwd: rows and pointers need 16-byte alignment");
   const Drop d = make_drop(p0, p1);
-  const int n_chunks = static_cast<int>((n_tok + kChunk - 1) / kChunk);
-  const int64_t groups = n_tok * (width / 8);
-  const int64_t want = (groups + 255) / 256, cap = static_cast<int64_t>(sm_count()) * 16;
+  const Split sp = split_of(n_tok, width);
+  const int n_units = sp.n_chunks * sp.col_blocks, n4 = width / 4 * rank * n_branch;
+  float* part = static_cast<float*>(workspace);
   return DECIK_DISPATCH_16(dtype, [&] {
-    dx_kernel<T><<<static_cast<int>(want < cap ? want : cap), 256, 0, s>>>(
-        static_cast<const T*>(du), ld_du, static_cast<const T*>(a), lda, addend, ld_add, dx, ld_dx, n_tok, width, rank,
-        n_branch, d, rng, stream_id);
-    float* part = static_cast<float*>(workspace);
-    const int n = rank * n_branch * width;
-    da_kernel<T><<<dim3((n / 8 + 255) / 256, n_chunks), 256, 0, s>>>(static_cast<const T*>(du), ld_du,
-                                                                     static_cast<const T*>(x16), ldx, part, n_tok,
-                                                                     width, rank, n_branch, d, rng, stream_id);
-    da_sum_kernel<<<(n + 255) / 256, 256, 0, s>>>(part, da, n_chunks, width, rank, n_branch, d);
+    auto go = [&](auto kernel) {
+      kernel<<<(n_units + 3) / 4, 128, 0, s>>>(static_cast<const T*>(du), ld_du, static_cast<const T*>(x16), ldx,
+                                               static_cast<const T*>(a), lda, addend, ld_add, dx, ld_dx, part, n_tok,
+                                               width, rank, sp.chunk, sp.col_blocks, n_units, d, rng, stream_id);
+    };
+    const int kr = (rank + 15) / 16;
+    if (n_branch == 2) kr == 1 ? go(bwd_kernel<T, 2, 1>) : go(bwd_kernel<T, 2, 2>);
+    else if (kr == 1) go(bwd_kernel<T, 1, 1>);
+    else kr == 2 ? go(bwd_kernel<T, 1, 2>) : go(bwd_kernel<T, 1, 4>);
+    da_sum_kernel<<<(n4 + 127) / 128, 128, 0, s>>>(part, da, sp.n_chunks, width, rank, n_branch, d);
     return check_launch("lora_down_dropout_bwd");
   });
 }

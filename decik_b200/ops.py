@@ -512,7 +512,7 @@ def lora_down_dropout_bwd(du: torch.Tensor, x16: torch.Tensor, a: torch.Tensor, 
         da = torch.empty((nb * rank, W), dtype=torch.float32, device=a.device)
         ws = torch.empty(int(lib.decik_lora_down_dropout_bwd_workspace(T, W, rank, nb)), dtype=torch.uint8,
                          device=a.device)
-        with _timed(what, 3):
+        with _timed(what, 2):
             rc = lib.decik_lora_down_dropout_bwd(
                 _p(du), _ld(du), _p(x16), _ld(x16), _p(a), _ld(a), _p(addend),
                 0 if addend is None else _ld(addend), _p(dx), _ld(dx), _p(da), T, W, rank, nb, ps[0], ps[1],
