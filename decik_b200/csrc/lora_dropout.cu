@@ -4,6 +4,8 @@
 //   forward   x16 = dt(x),  u_b = dt(s_b (keep_b o x16) A_b^T)
 //   backward  dx = addend + sum_b s_b keep_b o (du_b A_b),  dA_b = s_b du_b^T (keep_b o x16)
 // The index of x[t, k] is t * width + k (width % 8 == 0: a group of 8 stays in one row).
+#include <type_traits>
+
 #include "philox.cuh"
 #include "ptx.cuh"
 
@@ -13,33 +15,28 @@ namespace {
 
 constexpr int kMaxRank = 64;  // rows of A over all branches
 
-struct Drop {  // per branch
-  uint32_t cut[2];
+// per branch: a lane of the generator, in the high half of a word, is kept iff the word >= limit; a
+// scale of 0 means that nothing is kept (p = 1)
+struct Drop {
+  uint32_t limit[2];
   float scale[2];
 };
 
-// the kept values of a 16-bit pair v under the two lanes of one word of the generator
-__device__ __forceinline__ uint32_t mask_pair(uint32_t w, uint32_t v, uint32_t cut) {
-  const uint32_t m = ((w & 0xFFFFu) >= cut ? 0x0000FFFFu : 0u) | ((w >> 16) >= cut ? 0xFFFF0000u : 0u);
-  return v & m;
+// The kept values of a pair v of 16-bit values under one word of the generator. Predicated ands on two
+// compares: the shift runs on the FMA pipe, which leaves four instructions for the ALU pipe, the one
+// these kernels keep busiest.
+__device__ __forceinline__ bool keep_lo(uint32_t w, uint32_t limit) { return w * 65536u >= limit; }
+__device__ __forceinline__ bool keep_hi(uint32_t w, uint32_t limit) { return w >= limit; }
+__device__ __forceinline__ uint32_t mask_pair(uint32_t v, bool lo, bool hi) {
+  if (!lo) v &= 0xFFFF0000u;
+  if (!hi) v &= 0x0000FFFFu;
+  return v;
 }
-__device__ __forceinline__ void mask8(const uint4& w, const uint4& v, uint32_t cut, uint32_t (&m)[4]) {
-  m[0] = mask_pair(w.x, v.x, cut);
-  m[1] = mask_pair(w.y, v.y, cut);
-  m[2] = mask_pair(w.z, v.z, cut);
-  m[3] = mask_pair(w.w, v.w, cut);
-}
-
-// 8 consecutive values of x as 16-bit pairs
-template <typename T, typename X>
-__device__ __forceinline__ uint4 load8(const X* p) {
-  if constexpr (sizeof(X) == 2) {
-    return ldg16(p);
-  } else {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-    const float f[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-    return pack8<T>(f);
-  }
+__device__ __forceinline__ void mask8(const uint4& w, const uint4& v, uint32_t limit, uint32_t (&m)[4]) {
+  m[0] = mask_pair(v.x, keep_lo(w.x, limit), keep_hi(w.x, limit));
+  m[1] = mask_pair(v.y, keep_lo(w.y, limit), keep_hi(w.y, limit));
+  m[2] = mask_pair(v.z, keep_lo(w.z, limit), keep_hi(w.z, limit));
+  m[3] = mask_pair(v.w, keep_lo(w.w, limit), keep_hi(w.w, limit));
 }
 
 // transpose of an 8 x 8 matrix of 16-bit values held by a warp (lane 4 i + c: row i, columns 2 c, 2 c + 1)
@@ -52,22 +49,34 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
 // ------------------------------------------------------------------------------------------------
 // forward
 // ------------------------------------------------------------------------------------------------
-// A CTA takes 16 MT rows; its 8 warps share out the width in blocks of 32 columns and their partial
+// A CTA takes 16 MT rows; its warps share out the width in blocks of 32 columns and their partial
 // sums meet in shared memory. In a block, lane 4 g + c holds the 8 columns from 8 c of rows g and g + 8
 // (of each 16): 32 bytes of x in one go, one call of the generator per row and branch, and, because
 // the order of a sum's terms is free, an operand fragment of mma.sync m16n8k16 without any exchange:
 // the instruction's columns 2 c, 2 c + 1 and 2 c + 8, 2 c + 9 of step s are the lane's pairs 2 s and
 // 2 s + 1. lora_A's rows, read the same way (16 bytes of row g), are the other operand.
-constexpr int kWarps = 8;
-
+// The next block's bytes are on their way through cp.async while one is computed: a lane reads back
+// only what it copied itself, so shared memory serves as its registers and no barrier is needed.
 template <typename X, typename T, int NB, int NTB, int MT>
-__global__ void __launch_bounds__(32 * kWarps, NB * NTB <= 4 ? 2 : 1)
+struct DownTile {
+  static constexpr int kXPieces = sizeof(X) / 2;                       // 16-byte pieces of 8 columns
+  static constexpr int kPieces = MT * 2 * kXPieces + NB * NTB;         // of a lane, per block
+  static constexpr int kStage = kPieces * 512;                         // bytes of a warp's stage
+  static constexpr int kLd = 8 * NB * NTB + 4;                         // row of the partial sums
+  static constexpr int smem(int warps) {
+    const int ring = 2 * warps * kStage, red = warps * 16 * kLd * 4;
+    return ring > red ? ring : red;
+  }
+};
+
+template <typename X, typename T, int NB, int NTB, int MT, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS, NB * NTB <= 4 ? 16 / WARPS : 8 / WARPS)
 down_kernel(const X* __restrict__ x, int64_t ldx, const T* __restrict__ a, int64_t lda, T* __restrict__ x16,
             int64_t ldx16, T* __restrict__ u, int64_t ldu, int64_t n_tok, int width, int rank, Drop d,
             const int64_t* __restrict__ rng, int64_t stream_id) {
-  constexpr int NT = NB * NTB;            // n8 tiles of u's columns
-  constexpr int LD = 8 * NT + 4;
-  __shared__ float red[kWarps][16][LD];
+  using Tile = DownTile<X, T, NB, NTB, MT>;
+  constexpr int NT = NB * NTB, XP = Tile::kXPieces, LD = Tile::kLd;   // NT: n8 tiles of u's columns
+  extern __shared__ __align__(16) unsigned char smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * (16 * MT);
   philox::Key key[NB];
@@ -80,36 +89,66 @@ down_kernel(const X* __restrict__ x, int64_t ldx, const T* __restrict__ a, int64
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[m][n][e] = 0.f;
-  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-  for (int k = 32 * warp + 8 * c; k - 8 * c < width; k += 32 * kWarps) {
+  unsigned char* const ring = smem + warp * (2 * Tile::kStage) + lane * 16;
+  const int rows = n_tok - t0 < 16 * MT ? static_cast<int>(n_tok - t0) : 16 * MT;
+  // the lane's pieces of the block with its columns at k (zeros outside the matrix)
+  const X* const xp = x + (t0 + g) * ldx;
+  const T* const ap = a + static_cast<int64_t>(g) * lda;
+  auto issue = [&](int stage, int k) {
+    const uint32_t dst = ptx::smem_u32(ring) + stage * Tile::kStage;
     const bool in = k < width;
-    uint4 xv[MT][2];
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int i = 0; i < 2 * MT; ++i) {
+      const bool ok = in && 8 * i + g < rows;
+      const X* src = ok ? xp + 8 * i * ldx + k : x;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int64_t t = t0 + 16 * m + 8 * h + g;
-        xv[m][h] = in && t < n_tok ? load8<T>(x + t * ldx + k) : zero;
-      }
-    uint4 av[NT];
+      for (int j = 0; j < XP; ++j)
+        ptx::cp_async16(dst + (i * XP + j) * 512, reinterpret_cast<const char*>(src) + 16 * j, ok);
+    }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int r = 8 * (n % NTB);
-      av[n] = in && r < rank ? ldg16(a + static_cast<int64_t>(n / NTB * rank + r + g) * lda + k) : zero;
+      const bool ok = in && r < rank;
+      ptx::cp_async16(dst + (2 * MT * XP + n) * 512, ok ? ap + (n / NTB * rank + r) * lda + k : a, ok);
     }
+  };
+  int stage = 0;
+  const int step = 32 * WARPS;
+  const unsigned long long group0 = static_cast<unsigned long long>(t0 + g) * (width / 8);
+  if (32 * warp < width) issue(0, 32 * warp + 8 * c);
+  ptx::cp_async_commit();
+  for (int k = 32 * warp + 8 * c; k - 8 * c < width; k += step, stage ^= 1) {
+    __syncwarp();  // the other stage has been read
+    if (k - 8 * c + step < width) issue(stage ^ 1, k + step);
+    ptx::cp_async_commit();
+    ptx::cp_async_wait<1>();
+    __syncwarp();
+    const uint4* got = reinterpret_cast<const uint4*>(ring + stage * Tile::kStage);
+    uint4 av[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) av[n] = got[(2 * MT * XP + n) * 32];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
+      uint4 xv[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int64_t t = t0 + 16 * m + 8 * h + g;
-        if (x16 != nullptr && in && t < n_tok) stg16(x16 + t * ldx16 + k, xv[m][h]);
+        const uint4* p = got + (2 * m + h) * XP * 32;
+        if constexpr (XP == 1) {
+          xv[h] = p[0];
+        } else {
+          const float4 lo = *reinterpret_cast<const float4*>(p), hi = *reinterpret_cast<const float4*>(p + 32);
+          const float f[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+          xv[h] = pack8<T>(f);
+        }
+        if (x16 != nullptr && k < width && 16 * m + 8 * h + g < rows)
+          stg16(x16 + (t0 + 16 * m + 8 * h + g) * ldx16 + k, xv[h]);
       }
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         uint32_t lo[4], hi[4];
-        const unsigned long long group = static_cast<unsigned long long>(t0 + 16 * m + g) * (width / 8) + k / 8;
-        mask8(philox::words(key[b], group), xv[m][0], d.cut[b], lo);
-        mask8(philox::words(key[b], group + static_cast<unsigned long long>(width)), xv[m][1], d.cut[b], hi);
+        const unsigned long long group = group0 + static_cast<unsigned long long>(2 * m * width + k / 8);
+        mask8(philox::words(key[b], group), xv[0], d.limit[b], lo);
+        mask8(philox::words(key[b], group + static_cast<unsigned long long>(width)), xv[1], d.limit[b], hi);
         const uint32_t f0[4] = {lo[0], hi[0], lo[1], hi[1]}, f1[4] = {lo[2], hi[2], lo[3], hi[3]};
 #pragma unroll
         for (int n = b * NTB; n < (b + 1) * NTB; ++n) {
@@ -119,28 +158,32 @@ down_kernel(const X* __restrict__ x, int64_t ldx, const T* __restrict__ a, int64
       }
     }
   }
+  // the warps' sums in shared memory, over the ring
+  ptx::cp_async_wait<0>();
+  float* const red = reinterpret_cast<float*>(smem);  // [WARPS][16][LD]
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
-    if (m > 0) __syncthreads();
+    __syncthreads();
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      *reinterpret_cast<float2*>(&red[warp][g][8 * n + 2 * c]) = make_float2(acc[m][n][0], acc[m][n][1]);
-      *reinterpret_cast<float2*>(&red[warp][g + 8][8 * n + 2 * c]) = make_float2(acc[m][n][2], acc[m][n][3]);
+      float* const p = red + (warp * 16 + g) * LD + 8 * n + 2 * c;
+      *reinterpret_cast<float2*>(p) = make_float2(acc[m][n][0], acc[m][n][1]);
+      *reinterpret_cast<float2*>(p + 8 * LD) = make_float2(acc[m][n][2], acc[m][n][3]);
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < 16 * 4 * NT; i += 32 * kWarps) {  // a pair of u's columns
+    for (int i = threadIdx.x; i < 16 * 4 * NT; i += 32 * WARPS) {  // a pair of u's columns
       const int row = i / (4 * NT), col = 2 * (i % (4 * NT)), b = col / (8 * NTB), r = col % (8 * NTB);
       const int64_t t = t0 + 16 * m + row;
       if (t >= n_tok || r >= rank) continue;
       float2 s = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float2 v = *reinterpret_cast<const float2*>(&red[w][row][col]);
+      for (int w = 0; w < WARPS; ++w) {
+        const float2 v = *reinterpret_cast<const float2*>(red + (w * 16 + row) * LD + col);
         s.x += v.x;
         s.y += v.y;
       }
       const float scale = NB == 2 && b == 1 ? d.scale[1] : d.scale[0];
-      *reinterpret_cast<uint32_t*>(u + t * ldu + b * rank + r) = Dt<T>::pack2(s.x * scale, s.y * scale);
+      *reinterpret_cast<uint32_t*>(u + t * ldu + b * rank + r) = scale == 0.f ? 0u : Dt<T>::pack2(s.x * scale, s.y * scale);
     }
   }
 }
@@ -157,18 +200,27 @@ down_kernel(const X* __restrict__ x, int64_t ldx, const T* __restrict__ a, int64
 //       scale and addend are applied in place and dx leaves in 16-byte pieces;
 //   dA += du^T (keep x) (m = rank, k = token): the masked pair j of the lanes, as an 8 x 8 matrix
 //       (token, column), transposed by movmatrix is the operand fragment of tile j.
+// A tile's bytes are on their way two tiles ahead through cp.async into the warp's own ring.
+constexpr int kBwdStages = 3, kBwdWarps = 4;
+template <int NB, int KR>
+constexpr int bwd_stage() {  // x16: 2 pieces of 16 bytes a lane, the addend: 4, du: 16 tokens x 16 NB KR columns
+  return (2 + 4 + NB * KR) * 512;
+}
+
 template <typename T, int NB, int KR>
-__global__ void __launch_bounds__(128, NB * KR <= 2 ? 4 : 2)
+__global__ void __launch_bounds__(32 * kBwdWarps, NB * KR <= 2 ? 4 : 2)
 bwd_kernel(const T* __restrict__ du, int64_t ld_du, const T* __restrict__ x16, int64_t ldx, const T* __restrict__ a,
            int64_t lda, const float* addend, int64_t ld_add, float* dx, int64_t ld_dx, float* __restrict__ part,
            int64_t n_tok, int width, int rank, int chunk, int col_blocks, int n_units, Drop d,
            const int64_t* __restrict__ rng, int64_t stream_id) {
+  constexpr int kStage = bwd_stage<NB, KR>(), C = 2 * NB * KR;  // C: 16-byte pieces of a row of du
+  extern __shared__ __align__(16) unsigned char smem[];
   const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  const int unit = blockIdx.x * 4 + (threadIdx.x >> 5);  // (token chunk, block of 32 columns)
+  const int unit = blockIdx.x * kBwdWarps + (threadIdx.x >> 5);  // (token chunk, block of 32 columns)
   if (unit >= n_units) return;
   const int cb = unit % col_blocks;
   const int64_t first = static_cast<int64_t>(unit / col_blocks) * chunk;
-  const int64_t last = first + chunk < n_tok ? first + chunk : n_tok;
+  const int n = n_tok - first < chunk ? static_cast<int>(n_tok - first) : chunk;  // tokens of the chunk
   const int k = 32 * cb + 8 * c;
   const bool in = k < width;
   philox::Key key[NB];
@@ -196,52 +248,98 @@ bwd_kernel(const T* __restrict__ du, int64_t ld_du, const T* __restrict__ x16, i
         for (int e = 0; e < 4; ++e) acc[b][r][j][e] = 0.f;
       }
   }
-  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-  for (int64_t t0 = first; t0 < last; t0 += 16) {
-    const int64_t t[2] = {t0 + g, t0 + g + 8};
-    const bool ok[2] = {t[0] < last, t[1] < last};
-    uint4 xv[2];
-    float out[2][8];
-    uint32_t df[NB][KR][4];
+  unsigned char* const ring = smem + (threadIdx.x >> 5) * (kBwdStages * kStage);
+  const uint32_t ring_at = ptx::smem_u32(ring);
+  // running addresses: of the tile issued next, and of dx and the generator's group of the one computed
+  const T* xp = x16 + (first + g) * ldx + k;
+  const float* addp = addend != nullptr ? addend + (first + g) * ld_add + k : nullptr;
+  float* dxp = dx + (first + g) * ld_dx + k;
+  const T* dup[NB * KR];
+  uint32_t du_dst[NB * KR];
+  int du_row[NB * KR];  // past the chunk for a piece that is not there
+#pragma unroll
+  for (int q = 0; q < NB * KR; ++q) {  // du's rows, their pieces swizzled for ldmatrix
+    const int row = (lane + 32 * q) / C, piece = (lane + 32 * q) % C, b = piece / (2 * KR), r = 8 * (piece % (2 * KR));
+    dup[q] = du + (first + row) * ld_du + b * rank + r;
+    du_dst[q] = 6 * 512 + (row * C + (piece ^ (row * C / 8 & (C - 1)))) * 16;
+    du_row[q] = r < rank ? row : 1 << 30;
+  }
+  auto issue = [&](int stage, int i0) {
+    const uint32_t dst = ring_at + stage * kStage;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      xv[h] = ok[h] && in ? ldg16(x16 + t[h] * ldx + k) : zero;
-      float4 lo = make_float4(0.f, 0.f, 0.f, 0.f), hi = lo;
-      if (addend != nullptr && ok[h] && in) {
-        lo = *reinterpret_cast<const float4*>(addend + t[h] * ld_add + k);
-        hi = *reinterpret_cast<const float4*>(addend + t[h] * ld_add + k + 4);
-      }
-      out[h][0] = lo.x, out[h][1] = lo.y, out[h][2] = lo.z, out[h][3] = lo.w;
-      out[h][4] = hi.x, out[h][5] = hi.y, out[h][6] = hi.z, out[h][7] = hi.w;
+      const bool ok = in && i0 + 8 * h + g < n;
+      ptx::cp_async16(dst + h * 512 + lane * 16, ok ? xp + 8 * h * ldx : x16, ok);
+      if (addend == nullptr) continue;
+      const float* src = ok ? addp + 8 * h * ld_add : addend;
+      ptx::cp_async16(dst + (2 + 2 * h) * 512 + lane * 16, src, ok);
+      ptx::cp_async16(dst + (3 + 2 * h) * 512 + lane * 16, ok ? src + 4 : src, ok);
     }
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+    for (int q = 0; q < NB * KR; ++q) {
+      const bool ok = du_row[q] < n - i0;
+      ptx::cp_async16(dst + du_dst[q], ok ? dup[q] : du, ok);
+      dup[q] += 16 * ld_du;
+    }
+    xp += 16 * ldx;
+    addp += 16 * ld_add;
+  };
 #pragma unroll
-      for (int r = 0; r < KR; ++r)
+  for (int s = 0; s < kBwdStages - 1; ++s) {
+    if (16 * s < n) issue(s, 16 * s);
+    ptx::cp_async_commit();
+  }
+  int stage = 0;
+  unsigned long long group = static_cast<unsigned long long>(first + g) * (width / 8) + k / 8;
+  for (int i0 = 0; i0 < n; i0 += 16, group += 2 * width, dxp += 16 * ld_dx) {
+    ptx::cp_async_wait<kBwdStages - 2>();
+    __syncwarp();  // this stage has landed for every lane, and the one issued next has been read by all
+    const int ahead = i0 + 16 * (kBwdStages - 1);
+    if (ahead < n) issue(stage == 0 ? kBwdStages - 1 : stage - 1, ahead);
+    ptx::cp_async_commit();
+    const unsigned char* const got = ring + stage * kStage;
+    uint4 xv[2];
+    float out[2][8];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {  // (tokens g | g + 8, ranks 2 c .. | 2 c + 8 ..)
-          const int h = q & 1, row = 16 * r + 8 * (q >> 1) + 2 * c;
-          df[b][r][q] = ok[h] && row < rank
-                            ? __ldg(reinterpret_cast<const unsigned int*>(du + t[h] * ld_du + b * rank + row)) : 0u;
-        }
+    for (int h = 0; h < 2; ++h) {
+      xv[h] = *reinterpret_cast<const uint4*>(got + h * 512 + lane * 16);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) out[h][i] = 0.f;
+      if (addend != nullptr) {
+        const float4 lo = *reinterpret_cast<const float4*>(got + (2 + 2 * h) * 512 + lane * 16);
+        const float4 hi = *reinterpret_cast<const float4*>(got + (3 + 2 * h) * 512 + lane * 16);
+        out[h][0] = lo.x, out[h][1] = lo.y, out[h][2] = lo.z, out[h][3] = lo.w;
+        out[h][4] = hi.x, out[h][5] = hi.y, out[h][6] = hi.z, out[h][7] = hi.w;
+      }
+    }
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
+      if (d.scale[b] == 0.f) continue;  // nothing is kept
       uint32_t m[2][4];
-      float p[4][4];
+      float p[4][4] = {};
+      // rows (tokens) lane & 15, rank columns 8 (lane >> 4) ..
+      auto at = [&](int r) {
+        const int row = lane & 15, piece = 2 * (b * KR + r) + (lane >> 4);
+        return ring_at + stage * kStage + 6 * 512 + (row * C + (piece ^ (row * C / 8 & (C - 1)))) * 16;
+      };
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int r = 0; r < KR; ++r) {
+        uint32_t df[4];
+        ptx::ldsm_x4(at(r), df[0], df[1], df[2], df[3]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) p[j][e] = 0.f;
-#pragma unroll
-        for (int r = 0; r < KR; ++r) ptx::mma16816<T>(p[j], df[b][r], af[b][r][j][0], af[b][r][j][1]);
+        for (int j = 0; j < 4; ++j) ptx::mma16816<T>(p[j], df, af[b][r][j][0], af[b][r][j][1]);
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint4 w = philox::words(key[b], static_cast<unsigned long long>(t[h]) * (width / 8) + k / 8);
-        mask8(w, xv[h], d.cut[b], m[h]);
+        const uint4 w = philox::words(key[b], group + static_cast<unsigned long long>(h * width));
+        const uint32_t ws[4] = {w.x, w.y, w.z, w.w}, xs[4] = {xv[h].x, xv[h].y, xv[h].z, xv[h].w};
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (philox::keep_lane(w, i, d.cut[b])) out[h][i] += d.scale[b] * p[i >> 1][2 * h + (i & 1)];
+        for (int j = 0; j < 4; ++j) {
+          const bool lo = keep_lo(ws[j], d.limit[b]), hi = keep_hi(ws[j], d.limit[b]);
+          m[h][j] = mask_pair(xs[j], lo, hi);
+          if (lo) out[h][2 * j] = fmaf(d.scale[b], p[j][2 * h], out[h][2 * j]);
+          if (hi) out[h][2 * j + 1] = fmaf(d.scale[b], p[j][2 * h + 1], out[h][2 * j + 1]);
+        }
       }
       uint32_t bf[4][2];
 #pragma unroll
@@ -250,19 +348,20 @@ bwd_kernel(const T* __restrict__ du, int64_t ld_du, const T* __restrict__ x16, i
         for (int h = 0; h < 2; ++h) bf[j][h] = transpose8x8(m[h][j]);
 #pragma unroll
       for (int r = 0; r < KR; ++r) {
-        const uint32_t dt[4] = {transpose8x8(df[b][r][0]), transpose8x8(df[b][r][2]), transpose8x8(df[b][r][1]),
-                                transpose8x8(df[b][r][3])};
+        uint32_t dt[4];  // du^T: rows rank g | g + 8, columns tokens 2 c .. | 2 c + 8 ..
+        ptx::ldsm_x4_t(at(r), dt[0], dt[2], dt[1], dt[3]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) ptx::mma16816<T>(acc[b][r][j], dt, bf[j][0], bf[j][1]);
       }
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h)
-      if (ok[h] && in) {
-        float4* o = reinterpret_cast<float4*>(dx + t[h] * ld_dx + k);
+      if (in && i0 + 8 * h + g < n) {
+        float4* o = reinterpret_cast<float4*>(dxp + 8 * h * ld_dx);
         o[0] = make_float4(out[h][0], out[h][1], out[h][2], out[h][3]);
         o[1] = make_float4(out[h][4], out[h][5], out[h][6], out[h][7]);
       }
+    stage = stage + 1 == kBwdStages ? 0 : stage + 1;
   }
   if (!in) return;
 #pragma unroll
@@ -280,17 +379,27 @@ bwd_kernel(const T* __restrict__ du, int64_t ld_du, const T* __restrict__ x16, i
       }
 }
 
-// dA = scale * the sum of the chunks' partials, in chunk order (no atomics: the same bits every time)
-__global__ void __launch_bounds__(128)
-da_sum_kernel(const float* __restrict__ part, float* __restrict__ da, int n_chunks, int width, int rank, int branches,
-              Drop d) {
-  const int n4 = width / 4 * rank * branches, i = blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= n4) return;
-  const float4* p = reinterpret_cast<const float4*>(part) + i;
+// dA = scale * the sum of the chunks' partials in a fixed order (no atomics: the same bits every time):
+// warp w of a CTA sums chunks w, w + 8, ... of 128 values, then the warps' sums are added in order.
+__global__ void __launch_bounds__(256)
+da_sum_kernel(const float* __restrict__ part, float* __restrict__ da, int n_chunks, int width, int rank, Drop d, int n4) {
+  __shared__ float4 red[8][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i = blockIdx.x * 32 + lane;
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (i < n4) {
+    const float4* p = reinterpret_cast<const float4*>(part) + i;
 #pragma unroll 8
-  for (int c = 0; c < n_chunks; ++c) {
-    const float4 v = __ldg(p + static_cast<int64_t>(c) * n4);
+    for (int c = warp; c < n_chunks; c += 8) {
+      const float4 v = __ldg(p + static_cast<int64_t>(c) * n4);
+      s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+    }
+  }
+  red[warp][lane] = s;
+  __syncthreads();
+  if (warp != 0 || i >= n4) return;
+#pragma unroll
+  for (int w = 1; w < 8; ++w) {
+    const float4 v = red[w][lane];
     s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
   }
   const float scale = i / (width / 4) / rank == 1 ? d.scale[1] : d.scale[0];
@@ -332,9 +441,12 @@ int check_sizes(const char* what, int64_t n_tok, int width, int rank, int branch
 
 Drop make_drop(double p0, double p1) {
   Drop d;
-  d.cut[0] = philox::cut_of(p0);
-  d.cut[1] = philox::cut_of(p1);
-  for (int b = 0; b < 2; ++b) d.scale[b] = philox::scale_of(d.cut[b]);
+  const double p[2] = {p0, p1};
+  for (int b = 0; b < 2; ++b) {
+    const uint32_t cut = philox::cut_of(p[b]);
+    d.limit[b] = cut << 16;
+    d.scale[b] = philox::scale_of(cut);
+  }
   return d;
 }
 
@@ -354,16 +466,23 @@ struct DownArgs {
   cudaStream_t s;
 };
 
+template <typename X, typename T, int NB, int NTB, int MT, int WARPS>
+int launch_down_m(const DownArgs& p) {
+  static std::atomic<unsigned long long> done{0};
+  constexpr int smem = DownTile<X, T, NB, NTB, MT>::smem(WARPS);
+  auto kernel = down_kernel<X, T, NB, NTB, MT, WARPS>;
+  if (int rc = ensure_dyn_smem(kernel, smem, done, "lora_down_dropout")) return rc;
+  kernel<<<static_cast<unsigned>((p.n_tok + 16 * MT - 1) / (16 * MT)), 32 * WARPS, smem, p.s>>>(
+      static_cast<const X*>(p.x), p.ldx, static_cast<const T*>(p.a), p.lda, static_cast<T*>(p.x16), p.ldx16,
+      static_cast<T*>(p.u), p.ldu, p.n_tok, p.width, p.rank, p.d, p.rng, p.stream_id);
+  return check_launch("lora_down_dropout");
+}
+
+// Few rows: 16 a CTA, the width over 8 warps; many: 32 (lora_A is read half as often), over 4 warps.
 template <typename X, typename T, int NB, int NTB>
 int launch_down_t(const DownArgs& p) {
-  auto go = [&](auto kernel, int rows) {
-    kernel<<<static_cast<unsigned>((p.n_tok + rows - 1) / rows), 32 * kWarps, 0, p.s>>>(
-        static_cast<const X*>(p.x), p.ldx, static_cast<const T*>(p.a), p.lda, static_cast<T*>(p.x16), p.ldx16,
-        static_cast<T*>(p.u), p.ldu, p.n_tok, p.width, p.rank, p.d, p.rng, p.stream_id);
-  };
-  if (p.n_tok <= 32 * static_cast<int64_t>(sm_count())) go(down_kernel<X, T, NB, NTB, 1>, 16);
-  else go(down_kernel<X, T, NB, NTB, 2>, 32);
-  return check_launch("lora_down_dropout");
+  return p.n_tok <= 32 * static_cast<int64_t>(sm_count()) ? launch_down_m<X, T, NB, NTB, 1, 8>(p)
+                                                          : launch_down_m<X, T, NB, NTB, 2, 4>(p);
 }
 
 template <typename X, typename T>
@@ -433,16 +552,25 @@ extern "C" int decik_lora_down_dropout_bwd(const void* du, int64_t ld_du, const 
   const int n_units = sp.n_chunks * sp.col_blocks, n4 = width / 4 * rank * n_branch;
   float* part = static_cast<float*>(workspace);
   return DECIK_DISPATCH_16(dtype, [&] {
-    auto go = [&](auto kernel) {
-      kernel<<<(n_units + 3) / 4, 128, 0, s>>>(static_cast<const T*>(du), ld_du, static_cast<const T*>(x16), ldx,
-                                               static_cast<const T*>(a), lda, addend, ld_add, dx, ld_dx, part, n_tok,
-                                               width, rank, sp.chunk, sp.col_blocks, n_units, d, rng, stream_id);
+    auto go = [&](auto nb, auto kr) -> int {
+      static std::atomic<unsigned long long> done{0};
+      constexpr int smem = kBwdWarps * kBwdStages * bwd_stage<nb(), kr()>();
+      auto kernel = bwd_kernel<T, nb(), kr()>;
+      if (int rc = ensure_dyn_smem(kernel, smem, done, "lora_down_dropout_bwd")) return rc;
+      kernel<<<(n_units + kBwdWarps - 1) / kBwdWarps, 32 * kBwdWarps, smem, s>>>(
+          static_cast<const T*>(du), ld_du, static_cast<const T*>(x16), ldx, static_cast<const T*>(a), lda, addend,
+          ld_add, dx, ld_dx, part, n_tok, width, rank, sp.chunk, sp.col_blocks, n_units, d, rng, stream_id);
+      return check_launch("lora_down_dropout_bwd");
     };
+    using std::integral_constant;
+    const integral_constant<int, 1> one;
+    const integral_constant<int, 2> two;
+    const integral_constant<int, 4> four;
     const int kr = (rank + 15) / 16;
-    if (n_branch == 2) kr == 1 ? go(bwd_kernel<T, 2, 1>) : go(bwd_kernel<T, 2, 2>);
-    else if (kr == 1) go(bwd_kernel<T, 1, 1>);
-    else kr == 2 ? go(bwd_kernel<T, 1, 2>) : go(bwd_kernel<T, 1, 4>);
-    da_sum_kernel<<<(n4 + 127) / 128, 128, 0, s>>>(part, da, sp.n_chunks, width, rank, n_branch, d);
+    const int rc = n_branch == 2 ? (kr == 1 ? go(two, one) : go(two, two))
+                                 : kr == 1 ? go(one, one) : kr == 2 ? go(one, two) : go(one, four);
+    if (rc) return rc;
+    da_sum_kernel<<<(n4 + 31) / 32, 256, 0, s>>>(part, da, sp.n_chunks, width, rank, d, n4);
     return check_launch("lora_down_dropout_bwd");
   });
 }
