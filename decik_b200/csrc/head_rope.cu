@@ -9,7 +9,10 @@
 // The cosines come from fp32 tables [T, R] or, for several axes, from the token's positions:
 // angle j = position[axis of j] * inv_freq[j].
 //
-// All arithmetic is fp32 with one rounding at the end. HBM-bound.
+// All arithmetic is fp32 with one rounding at the end. HBM-bound. L lanes hold a token's row of D values,
+// 16 each, and walk over its heads: the angles (read from the tables or computed), with the weights
+// folded in, stay in registers for all of them, a row's mean square is log2 L shuffles, and a lane's two
+// 16-byte pieces are rotation partners.
 #include "common.cuh"
 
 namespace decik {
@@ -22,7 +25,7 @@ struct Angles {
   const float* cos;
   const float* sin;
   const void* pos;
-  int pos32;
+  int pos32, n_axes;
   int64_t ld_pos;
   const float* inv_freq;
   uint32_t axis[8];
@@ -68,9 +71,9 @@ __device__ __forceinline__ double position(const Angles& a, int axis, int64_t t)
                  : static_cast<double>(__ldg(static_cast<const long long*>(a.pos) + i));
 }
 
-// A row of D values is held by L lanes (the power of two at or above D / 16), 16 values each: lane c
-// holds the 8 values from lo and the 8 from hi. Lanes below R / 16 hold rotation partners (hi = lo +
-// R / 2), those below D / 16 the values behind R, the rest nothing.
+// A row of D values is held by L lanes (4, 8 or 16: a power of two at or above D / 16), 16 values each:
+// lane c holds the 8 values from lo and the 8 from hi. Lanes below R / 16 hold rotation partners (hi = lo
+// + R / 2), those below D / 16 the values behind R, the rest nothing.
 struct Lane {
   int lo, hi;
   bool active, rot;
@@ -84,57 +87,49 @@ __device__ __forceinline__ Lane lane_of(int c, int D, int R) {
   return l;
 }
 
+__device__ __forceinline__ void load8f(const float* p, float (&f)[8]) {
+  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+  f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+}
+
+// cos and sin of the lane's values at token t: of its lo and hi values from tables, of its frequencies
+// (the same for both) from positions; 1 and 0 for values that are not rotated. N = 8 or 16.
 template <bool AXES>
-__device__ __forceinline__ void load_angles(const Args& p, const Lane& l, int64_t t, float (&cl)[8], float (&ch)[8],
-                                            float (&sl)[8], float (&sh)[8]) {
+__device__ __forceinline__ void load_angles(const Args& p, const Lane& l, bool ok, int64_t t,
+                                            float (&c)[AXES ? 8 : 16], float (&s)[AXES ? 8 : 16]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    cl[i] = ch[i] = 1.f;
-    sl[i] = sh[i] = 0.f;
-    if (!l.rot) continue;
-    if constexpr (AXES) {
-      const int j = l.lo + i;
-      sincos_of(position(p.ang, (p.ang.axis[j >> 4] >> (2 * (j & 15))) & 3, t), __ldg(p.ang.inv_freq + j), sl[i], cl[i]);
-      ch[i] = cl[i];
-      sh[i] = sl[i];
-    } else {
-      cl[i] = __ldg(p.ang.cos + t * p.R + l.lo + i);
-      ch[i] = __ldg(p.ang.cos + t * p.R + l.hi + i);
-      sl[i] = __ldg(p.ang.sin + t * p.R + l.lo + i);
-      sh[i] = __ldg(p.ang.sin + t * p.R + l.hi + i);
+  for (int i = 0; i < (AXES ? 8 : 16); ++i) c[i] = 1.f, s[i] = 0.f;
+  if (!ok || !l.rot) return;
+  if constexpr (AXES) {
+    double pos[4];
+#pragma unroll
+    for (int a = 0; a < 4; ++a) pos[a] = a < p.ang.n_axes ? position(p.ang, a, t) : 0.0;
+    float f[8];
+    load8f(p.ang.inv_freq + l.lo, f);
+    const uint32_t map = p.ang.axis[l.lo >> 4] >> (2 * (l.lo & 15));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int axis = (map >> (2 * i)) & 3;
+      const double x = axis & 2 ? (axis & 1 ? pos[3] : pos[2]) : (axis & 1 ? pos[1] : pos[0]);
+      sincos_of(x, f[i], s[i], c[i]);
     }
+  } else {
+    float v[4][8];
+    load8f(p.ang.cos + t * p.R + l.lo, v[0]);
+    load8f(p.ang.cos + t * p.R + l.hi, v[1]);
+    load8f(p.ang.sin + t * p.R + l.lo, v[2]);
+    load8f(p.ang.sin + t * p.R + l.hi, v[3]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = v[0][i], c[8 + i] = v[1][i], s[i] = v[2][i], s[8 + i] = v[3][i];
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void load_row(const decik_tensor3& x, const Lane& l, int64_t t, int h, float (&lo)[8],
-                                         float (&hi)[8]) {
-  const T* p = static_cast<const T*>(x.ptr) + t * x.tok_stride + h * x.head_stride;
-  unpack8<T>(ldg16(p + l.lo), lo);
-  unpack8<T>(ldg16(p + l.hi), hi);
-}
-template <typename T>
-__device__ __forceinline__ void store_row(const decik_tensor3_mut& x, const Lane& l, int64_t t, int h,
-                                          const float (&lo)[8], const float (&hi)[8]) {
-  T* p = static_cast<T*>(x.ptr) + t * x.tok_stride + h * x.head_stride;
-  stg16(p + l.lo, pack8<T>(lo));
-  stg16(p + l.hi, pack8<T>(hi));
-}
-// the row's x (with the LoRA delta of the queries added in fp32); zeros in lanes that hold nothing
-template <typename T>
-__device__ __forceinline__ void load_x(const Args& p, const Lane& l, int64_t t, int h, float (&lo)[8], float (&hi)[8]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) lo[i] = hi[i] = 0.f;
-  if (!l.active) return;
-  if (h >= p.hq) return load_row<T>(p.k, l, t, h - p.hq, lo, hi);
-  load_row<T>(p.q, l, t, h, lo, hi);
-  if (p.ql.ptr == nullptr) return;
-  float a[8], b[8];
-  load_row<T>(p.ql, l, t, h, a, b);
+// the lane's 16 weights (lo, then hi); zeros in lanes that hold nothing
+__device__ __forceinline__ void load_weights(const void* w, int dtype, const Lane& l, float (&v)[16]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    lo[i] += a[i];
-    hi[i] += b[i];
+    v[i] = l.active ? load_w(w, dtype, l.lo + i) : 0.f;
+    v[8 + i] = l.active ? load_w(w, dtype, l.hi + i) : 0.f;
   }
 }
 
@@ -145,163 +140,269 @@ __device__ __forceinline__ float row_sum(float v) {
   return v;
 }
 
-template <typename T, int L, bool NORM, bool AXES>
-__global__ void __launch_bounds__(256) fwd_kernel(const Args p, int w_dtype) {
-  const int heads = p.hq + p.hk;
-  const int64_t rows = p.n_tok * heads, per_grid = static_cast<int64_t>(gridDim.x) * (256 / L);
+struct Raw {  // a lane's 16 values of a row as they lie in memory
+  uint4 lo, hi;
+};
+template <typename T>
+__device__ __forceinline__ Raw load_raw(const T* p, const Lane& l, bool ok) {
+  Raw r{make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
+  if (ok) {
+    r.lo = ldg16(p + l.lo);
+    r.hi = ldg16(p + l.hi);
+  }
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void unpack(const Raw& r, float (&x)[16]) {
+  float a[8], b[8];
+  unpack8<T>(r.lo, a);
+  unpack8<T>(r.hi, b);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = a[i], x[8 + i] = b[i];
+}
+template <typename T>
+__device__ __forceinline__ void add(const Raw& r, float (&x)[16]) {
+  float y[16];
+  unpack<T>(r, y);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] += y[i];
+}
+template <typename T>
+__device__ __forceinline__ void store(T* p, const Lane& l, const float (&x)[16]) {
+  float a[8], b[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) a[i] = x[i], b[i] = x[8 + i];
+  stg16(p + l.lo, pack8<T>(a));
+  stg16(p + l.hi, pack8<T>(b));
+}
+
+constexpr int kThreads = 128;
+
+// Forward; with sign -1 and without norms also the backward (the rotation by the opposite angle).
+// Block (x, y): 128 / L tokens, heads y * per_group .. of the queries' and then the keys' heads. The
+// loads of U heads are in flight together.
+template <typename T, int L, bool NORM, bool AXES, bool LORA>
+__global__ void __launch_bounds__(kThreads) fwd_kernel(const Args p, int w_dtype, int per_group, float sign) {
+  constexpr int U = LORA ? 2 : 4;
   const Lane l = lane_of(threadIdx.x % L, p.D, p.R);
-  // every lane of a warp takes every step: the row sums are warp shuffles
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * (256 / L) + threadIdx.x / L;
-  for (int64_t base = 0; base < rows; base += per_grid) {
-    const int64_t row = base + first;
-    const bool ok = row < rows && l.active;
-    const int64_t t = ok ? row / heads : 0;
-    const int h = ok ? static_cast<int>(row % heads) : 0;
-    float lo[8], hi[8];
-    load_x<T>(p, l, t, h, lo, hi);
-    if constexpr (NORM) {
-      float ss = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) ss += lo[i] * lo[i] + hi[i] * hi[i];
-      const float r = rsqrtf(row_sum<L>(ss) / p.D + p.eps);
-      const void* w = h < p.hq ? p.wq : p.wk;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        lo[i] *= r * (l.active ? load_w(w, w_dtype, l.lo + i) : 0.f);
-        hi[i] *= r * (l.active ? load_w(w, w_dtype, l.hi + i) : 0.f);
-      }
-    }
-    if (!ok) continue;
-    float cl[8], ch[8], sl[8], sh[8], ol[8], oh[8];
-    load_angles<AXES>(p, l, t, cl, ch, sl, sh);
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * (kThreads / L) + threadIdx.x / L;
+  const bool ok = t < p.n_tok && l.active;
+  const int h0 = blockIdx.y * per_group, h1 = h0 + per_group < p.hq + p.hk ? h0 + per_group : p.hq + p.hk;
+  float cs[AXES ? 8 : 16], sn[AXES ? 8 : 16];
+  load_angles<AXES>(p, l, ok, t, cs, sn);
+#pragma unroll 1
+  for (int part = 0; part < 2; ++part) {  // queries, keys
+    const int first = part ? (h0 > p.hq ? h0 - p.hq : 0) : h0, last = part ? h1 - p.hq : (h1 < p.hq ? h1 : p.hq);
+    if (first >= last) continue;
+    const decik_tensor3& in = part ? p.k : p.q;
+    const decik_tensor3_mut& out = part ? p.ok : p.oq;
+    // out[lo] = r (x[lo] m[0] - x[hi] m[1]), out[hi] = r (x[hi] m[2] + x[lo] m[3])
+    float m[4][8], w[16];
+    if constexpr (NORM) load_weights(part ? p.wk : p.wq, w_dtype, l, w);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      ol[i] = lo[i] * cl[i] - hi[i] * sl[i];
-      oh[i] = hi[i] * ch[i] + lo[i] * sh[i];
+      const int hi = AXES ? i : 8 + i;
+      m[0][i] = NORM ? w[i] * cs[i] : cs[i];
+      m[1][i] = sign * (NORM ? w[8 + i] * sn[i] : sn[i]);
+      m[2][i] = NORM ? w[8 + i] * cs[hi] : cs[hi];
+      m[3][i] = sign * (NORM ? w[i] * sn[hi] : sn[hi]);
     }
-    if (h < p.hq) store_row<T>(p.oq, l, t, h, ol, oh);
-    else store_row<T>(p.ok, l, t, h - p.hq, ol, oh);
+    const T* src = static_cast<const T*>(in.ptr) + t * in.tok_stride + first * in.head_stride;
+    const T* lora = LORA && !part ? static_cast<const T*>(p.ql.ptr) + t * p.ql.tok_stride + first * p.ql.head_stride : src;
+    const int64_t lora_hs = LORA && !part ? p.ql.head_stride : 0;
+    T* dst = static_cast<T*>(out.ptr) + t * out.tok_stride + first * out.head_stride;
+    for (int h = first; h < last; h += U) {
+      Raw raw[U], rl[LORA ? U : 1];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        raw[u] = load_raw(src + u * in.head_stride, l, ok && h + u < last);
+        if constexpr (LORA) rl[u] = load_raw(lora + u * lora_hs, l, ok && !part && h + u < last);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (h + u >= last) break;
+        float x[16], o[16], r = 1.f;
+        unpack<T>(raw[u], x);
+        if constexpr (LORA) add<T>(rl[u], x);
+        if constexpr (NORM) {
+          float ss = 0.f;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) ss += x[i] * x[i];
+          r = rsqrtf(row_sum<L>(ss) / p.D + p.eps);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[i] *= r;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          o[i] = x[i] * m[0][i] - x[8 + i] * m[1][i];
+          o[8 + i] = x[8 + i] * m[2][i] + x[i] * m[3][i];
+        }
+        if (ok) store(dst + u * out.head_stride, l, o);
+      }
+      src += U * in.head_stride;
+      lora += U * lora_hs;
+      dst += U * out.head_stride;
+    }
   }
 }
 
-// The weight gradients are summed in fp32: a thread's own rows (queries, then keys), then the CTA's
-// threads that hold the same values, in shared memory, then the CTAs in a kernel of their own, all
-// in a fixed order.
-template <typename T, int L, bool NORM, bool AXES>
-__global__ void __launch_bounds__(256) bwd_kernel(const Args p, int w_dtype) {
-  __shared__ float red[NORM ? 256 * 17 : 1];
-  const Lane l = lane_of(threadIdx.x % L, p.D, p.R);
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * (256 / L) + threadIdx.x / L;
-  const int64_t per_grid = static_cast<int64_t>(gridDim.x) * (256 / L);
-  for (int part = 0; part < 2; ++part) {  // queries, keys
-    const int heads = part ? p.hk : p.hq;
-    const int64_t rows = p.n_tok * heads;
-    const void* w = part ? p.wk : p.wq;
-    float dwl[8] = {}, dwh[8] = {};
-    for (int64_t base = 0; base < rows; base += per_grid) {
-      const int64_t row = base + first;
-      const bool ok = row < rows && l.active;
-      const int64_t t = ok ? row / heads : 0;
-      const int h = ok ? static_cast<int>(row % heads) : 0;
-      float gl[8], gh[8], cl[8], ch[8], sl[8], sh[8], zl[8], zh[8];
+// The backward with norms. A CTA walks over tiles of 128 / L tokens; a head's row is read while the one
+// before is computed. The weight gradients are summed in fp32: a lane's own rows (the queries' in
+// registers, the keys', which are fewer, in a slot of its own in shared memory), then the CTA's lanes
+// that hold the same values, then the CTAs in a kernel of their own, all in a fixed order.
+template <typename T, int L, bool AXES, bool LORA>
+__global__ void __launch_bounds__(kThreads) norm_bwd_kernel(const Args p, int w_dtype, int64_t n_tiles) {
+  __shared__ float red[2][kThreads][17];
+  __shared__ float ws[2][16][L];  // weights of lane c: ws[part][i][c]
+  const int c = threadIdx.x % L;
+  const Lane l = lane_of(c, p.D, p.R);
+  if (threadIdx.x < 2 * L) {
+    float w[16];
+    load_weights(threadIdx.x < L ? p.wq : p.wk, w_dtype, l, w);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) gl[i] = gh[i] = 0.f;
-      if (ok) load_row<T>(part ? p.gk : p.gq, l, t, h, gl, gh);
-      load_angles<AXES>(p, l, t, cl, ch, sl, sh);
+    for (int i = 0; i < 16; ++i) ws[threadIdx.x / L][i][c] = w[i];
+  }
+  float dw[16] = {};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        zl[i] = gl[i] * cl[i] + gh[i] * sh[i];
-        zh[i] = gh[i] * ch[i] - gl[i] * sl[i];
-      }
-      if constexpr (NORM) {
-        float xl[8], xh[8];
-        load_x<T>(p, l, t, part ? p.hq + h : h, xl, xh);
+  for (int i = 0; i < 16; ++i) red[1][threadIdx.x][i] = 0.f;
+  __syncthreads();
+  for (int64_t tile = blockIdx.x; tile < n_tiles; tile += gridDim.x) {
+    const int64_t t = tile * (kThreads / L) + threadIdx.x / L;
+    const bool ok = t < p.n_tok && l.active;
+    float cs[AXES ? 8 : 16], sn[AXES ? 8 : 16];
+    load_angles<AXES>(p, l, ok, t, cs, sn);
+#pragma unroll 1
+    for (int part = 0; part < 2; ++part) {
+      const decik_tensor3& gr = part ? p.gk : p.gq;
+      const decik_tensor3& in = part ? p.k : p.q;
+      const decik_tensor3_mut& out = part ? p.ok : p.oq;
+      const int heads = part ? p.hk : p.hq;
+      const T* g = static_cast<const T*>(gr.ptr) + t * gr.tok_stride;
+      const T* src = static_cast<const T*>(in.ptr) + t * in.tok_stride;
+      const T* lora = static_cast<const T*>(p.ql.ptr) + t * p.ql.tok_stride;
+      T* dst = static_cast<T*>(out.ptr) + t * out.tok_stride;
+      const bool has_lora = LORA && !part;
+      Raw rg = load_raw(g, l, ok), rx = load_raw(src, l, ok), rl;
+      if constexpr (LORA) rl = load_raw(lora, l, ok && has_lora);
+      for (int h = 0; h < heads; ++h) {
+        float x[16], gv[16], z[16];
+        unpack<T>(rg, gv);
+        unpack<T>(rx, x);
+        if constexpr (LORA) add<T>(rl, x);
+        const bool next = ok && h + 1 < heads;
+        g += gr.head_stride;
+        src += in.head_stride;
+        lora += p.ql.head_stride;
+        rg = load_raw(g, l, next);
+        rx = load_raw(src, l, next);
+        if constexpr (LORA) rl = load_raw(lora, l, next && has_lora);
         float ss = 0.f, zx = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ss += xl[i] * xl[i] + xh[i] * xh[i];
-        const float r = rsqrtf(row_sum<L>(ss) / p.D + p.eps);
-#pragma unroll
         for (int i = 0; i < 8; ++i) {
-          if (ok) {
-            dwl[i] += zl[i] * xl[i] * r;
-            dwh[i] += zh[i] * xh[i] * r;
-          }
-          zl[i] *= l.active ? load_w(w, w_dtype, l.lo + i) : 0.f;
-          zh[i] *= l.active ? load_w(w, w_dtype, l.hi + i) : 0.f;
-          zx += zl[i] * xl[i] + zh[i] * xh[i];
+          const int hi = AXES ? i : 8 + i;
+          z[i] = gv[i] * cs[i] + gv[8 + i] * sn[hi];
+          z[8 + i] = gv[8 + i] * cs[hi] - gv[i] * sn[i];
         }
-        const float m = r * r * row_sum<L>(zx) / p.D;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          zl[i] = r * (zl[i] - xl[i] * m);
-          zh[i] = r * (zh[i] - xh[i] * m);
+        for (int i = 0; i < 16; ++i) ss += x[i] * x[i];
+        // (of a row that is not there 0, so that it adds nothing to the sums with eps = 0 either)
+        const float rs = rsqrtf(row_sum<L>(ss) / p.D + p.eps), r = t < p.n_tok ? rs : 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          x[i] *= r;
+          const float d = z[i] * x[i];
+          if (part) red[1][threadIdx.x][i] += d;
+          else dw[i] += d;
+          const float w = ws[part][i][c];
+          zx += d * w;
+          z[i] *= w;
         }
-      }
-      if (ok) store_row<T>(part ? p.ok : p.oq, l, t, h, zl, zh);
-    }
-    if constexpr (NORM) {
-      __syncthreads();
+        const float mean = row_sum<L>(zx) / p.D;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        red[threadIdx.x * 17 + i] = dwl[i];
-        red[threadIdx.x * 17 + 8 + i] = dwh[i];
-      }
-      __syncthreads();
-      if (threadIdx.x < 16 * L) {  // value i of lane c over the CTA's rows
-        const int c = threadIdx.x / 16, i = threadIdx.x % 16;
-        const Lane o = lane_of(c, p.D, p.R);
-        float s = 0.f;
-        for (int k = c; k < 256; k += L) s += red[k * 17 + i];
-        if (o.active) p.part[(2 * static_cast<int64_t>(blockIdx.x) + part) * p.D + (i < 8 ? o.lo + i : o.hi + i - 8)] = s;
+        for (int i = 0; i < 16; ++i) z[i] = r * (z[i] - x[i] * mean);
+        if (ok) store(dst, l, z);
+        dst += out.head_stride;
       }
     }
   }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) red[0][threadIdx.x][i] = dw[i];
+  __syncthreads();
+  for (int j = threadIdx.x; j < 2 * 16 * L; j += kThreads) {  // value i of lane k over the CTA's rows
+    const int part = j / (16 * L), k = j / 16 % L, i = j % 16;
+    const Lane o = lane_of(k, p.D, p.R);
+    float s = 0.f;
+    for (int n = k; n < kThreads; n += L) s += red[part][n][i];
+    if (o.active) p.part[(2 * static_cast<int64_t>(blockIdx.x) + part) * p.D + (i < 8 ? o.lo + i : o.hi + i - 8)] = s;
+  }
 }
 
-// dw[d] = the sum of the CTAs' partials, in CTA order
-__global__ void __launch_bounds__(256) dw_sum_kernel(const float* __restrict__ part, float* __restrict__ dwq,
-                                                     float* __restrict__ dwk, int n_part, int D) {
-  const int i = blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= 2 * D) return;
+// dw[d] = the sum of the CTAs' partials in a fixed order: thread (d, j) of a block sums CTAs j, j + 32, ...
+// for one of its 32 values, then the 32 sums are added in order.
+__global__ void __launch_bounds__(1024) dw_sum_kernel(const float* __restrict__ part, float* __restrict__ dwq,
+                                                      float* __restrict__ dwk, int n_part, int D) {
+  __shared__ float red[32][33];
+  const int d = blockIdx.x * 32 + (threadIdx.x & 31), j = threadIdx.x >> 5;  // 2 D is a multiple of 32
   float s = 0.f;
-  for (int c = 0; c < n_part; ++c) s += part[static_cast<int64_t>(c) * 2 * D + i];
-  (i < D ? dwq : dwk)[i < D ? i : i - D] = s;
+#pragma unroll 8
+  for (int c = j; c < n_part; c += 32) s += __ldg(part + static_cast<int64_t>(c) * 2 * D + d);
+  red[j][threadIdx.x & 31] = s;
+  __syncthreads();
+  if (j != 0) return;
+  for (int k = 1; k < 32; ++k) s += red[k][threadIdx.x];
+  (d < D ? dwq : dwk)[d < D ? d : d - D] = s;
 }
 
-int lanes_of(int D) {
-  int l = 1;
-  while (16 * l < D) l *= 2;
-  return l;
-}
+int lanes_of(int D) { return D <= 64 ? 4 : D <= 128 ? 8 : 16; }
 
 constexpr int kMaxPart = 2048;  // CTAs of a backward pass with norms
 
-int grid_of(int64_t rows, int D, int per_sm) {
-  const int64_t want = (rows * lanes_of(D) + 255) / 256, cap = static_cast<int64_t>(sm_count()) * per_sm;
-  return static_cast<int>(want < 1 ? 1 : want < cap ? want : cap);
-}
-
-template <typename T, int L, bool BWD>
-int launch_l(const Args& p, bool norm, bool axes, int w_dtype, int grid, cudaStream_t s) {
-  auto go = [&](auto kernel) { kernel<<<grid, 256, 0, s>>>(p, w_dtype); };
-  if constexpr (BWD) {
-    if (norm) axes ? go(bwd_kernel<T, L, true, true>) : go(bwd_kernel<T, L, true, false>);
-    else go(bwd_kernel<T, L, false, true>);
+template <typename T, int L>
+int launch_fwd_l(const Args& p, bool norm, bool axes, int w_dtype, float sign, cudaStream_t s) {
+  const int64_t tiles = (p.n_tok + kThreads / L - 1) / (kThreads / L);
+  // few tokens: the heads of a token over several CTAs, until there are four for every SM
+  const int heads = p.hq + p.hk;
+  int64_t groups = 4 * static_cast<int64_t>(sm_count()) / tiles;
+  groups = groups < 1 ? 1 : groups > heads ? heads : groups;
+  const int per_group = static_cast<int>((heads + groups - 1) / groups);
+  const dim3 grid(static_cast<unsigned>(tiles), (heads + per_group - 1) / per_group);
+  auto go = [&](auto kernel) { kernel<<<grid, kThreads, 0, s>>>(p, w_dtype, per_group, sign); };
+  const bool lora = p.ql.ptr != nullptr;
+  if (norm) {
+    if (axes) lora ? go(fwd_kernel<T, L, true, true, true>) : go(fwd_kernel<T, L, true, true, false>);
+    else lora ? go(fwd_kernel<T, L, true, false, true>) : go(fwd_kernel<T, L, true, false, false>);
   } else {
-    if (norm) axes ? go(fwd_kernel<T, L, true, true>) : go(fwd_kernel<T, L, true, false>);
-    else go(fwd_kernel<T, L, false, true>);
+    lora ? go(fwd_kernel<T, L, false, true, true>) : go(fwd_kernel<T, L, false, true, false>);
   }
-  return check_launch(BWD ? "head_rope_bwd" : "head_rope_fwd");
+  return check_launch("head_rope_fwd");
 }
 
-template <typename T, bool BWD>
-int launch(const Args& p, bool norm, bool axes, int w_dtype, int grid, cudaStream_t s) {
+template <typename T, int L>
+int launch_bwd_l(const Args& p, bool axes, int w_dtype, int* n_part, cudaStream_t s) {
+  const int64_t tiles = (p.n_tok + kThreads / L - 1) / (kThreads / L), cap = static_cast<int64_t>(sm_count()) * 4;
+  const int grid = static_cast<int>(tiles < cap ? tiles : cap < kMaxPart ? cap : kMaxPart);
+  *n_part = grid;
+  auto go = [&](auto kernel) { kernel<<<grid, kThreads, 0, s>>>(p, w_dtype, tiles); };
+  const bool lora = p.ql.ptr != nullptr;
+  if (axes) lora ? go(norm_bwd_kernel<T, L, true, true>) : go(norm_bwd_kernel<T, L, true, false>);
+  else lora ? go(norm_bwd_kernel<T, L, false, true>) : go(norm_bwd_kernel<T, L, false, false>);
+  return check_launch("head_rope_bwd");
+}
+
+template <typename T>
+int launch_fwd(const Args& p, bool norm, bool axes, int w_dtype, float sign, cudaStream_t s) {
   switch (lanes_of(p.D)) {
-    case 1: return launch_l<T, 1, BWD>(p, norm, axes, w_dtype, grid, s);
-    case 2: return launch_l<T, 2, BWD>(p, norm, axes, w_dtype, grid, s);
-    case 4: return launch_l<T, 4, BWD>(p, norm, axes, w_dtype, grid, s);
-    case 8: return launch_l<T, 8, BWD>(p, norm, axes, w_dtype, grid, s);
-    default: return launch_l<T, 16, BWD>(p, norm, axes, w_dtype, grid, s);
+    case 4: return launch_fwd_l<T, 4>(p, norm, axes, w_dtype, sign, s);
+    case 8: return launch_fwd_l<T, 8>(p, norm, axes, w_dtype, sign, s);
+    default: return launch_fwd_l<T, 16>(p, norm, axes, w_dtype, sign, s);
+  }
+}
+template <typename T>
+int launch_bwd(const Args& p, bool axes, int w_dtype, int* n_part, cudaStream_t s) {
+  switch (lanes_of(p.D)) {
+    case 4: return launch_bwd_l<T, 4>(p, axes, w_dtype, n_part, s);
+    case 8: return launch_bwd_l<T, 8>(p, axes, w_dtype, n_part, s);
+    default: return launch_bwd_l<T, 16>(p, axes, w_dtype, n_part, s);
   }
 }
 
@@ -348,6 +449,7 @@ int set_axes(const char* what, Args& p, const void* positions, int pos_dtype, in
     return set_error(DECIK_ERR_INVALID, "%s: null pointer, or rows of positions shorter than the tokens", what);
   p.ang.pos = positions;
   p.ang.pos32 = pos_dtype;
+  p.ang.n_axes = n_axes;
   p.ang.ld_pos = ld_pos;
   p.ang.inv_freq = inv_freq;
   for (int j = 0; j < 8; ++j) p.ang.axis[j] = 0;
@@ -362,8 +464,7 @@ int set_axes(const char* what, Args& p, const void* positions, int pos_dtype, in
 int run_fwd(const char* what, const Args& p, bool axes, int w_dtype, int dtype, cudaStream_t s) {
   if (int rc = check(what, p, p.wq != nullptr, false, w_dtype, dtype)) return rc;
   if (p.n_tok == 0) return DECIK_OK;
-  const int grid = grid_of(p.n_tok * (p.hq + p.hk), p.D, 16);
-  return DECIK_DISPATCH_16(dtype, [&] { return launch<T, false>(p, p.wq != nullptr, axes, w_dtype, grid, s); });
+  return DECIK_DISPATCH_16(dtype, [&] { return launch_fwd<T>(p, p.wq != nullptr, axes, w_dtype, 1.f, s); });
 }
 
 int run_bwd(const char* what, Args p, bool axes, int w_dtype, float* dwq, float* dwk, void* workspace, int dtype,
@@ -379,12 +480,16 @@ int run_bwd(const char* what, Args p, bool axes, int w_dtype, float* dwq, float*
   }
   if (norm && (!workspace || !aligned16(workspace)))
     return set_error(DECIK_ERR_INVALID, "%s: workspace NULL or not 16-byte aligned", what);
+  if (!norm) {  // the rotation back, from the gradients
+    p.q = p.gq;
+    p.k = p.gk;
+    p.ql = {};
+    return DECIK_DISPATCH_16(dtype, [&] { return launch_fwd<T>(p, false, axes, w_dtype, -1.f, s); });
+  }
   p.part = static_cast<float*>(workspace);
-  int grid = grid_of(p.n_tok * p.hq, p.D, 4);
-  if (grid > kMaxPart) grid = kMaxPart;
-  if (int rc = DECIK_DISPATCH_16(dtype, [&] { return launch<T, true>(p, norm, axes, w_dtype, grid, s); })) return rc;
-  if (!norm) return DECIK_OK;
-  dw_sum_kernel<<<(2 * p.D + 255) / 256, 256, 0, s>>>(p.part, dwq, dwk, grid, p.D);
+  int n_part = 0;
+  if (int rc = DECIK_DISPATCH_16(dtype, [&] { return launch_bwd<T>(p, axes, w_dtype, &n_part, s); })) return rc;
+  dw_sum_kernel<<<2 * p.D / 32, 1024, 0, s>>>(p.part, dwq, dwk, n_part, p.D);
   return check_launch(what);
 }
 
