@@ -14,6 +14,7 @@
 // folded in, stay in registers for all of them, a row's mean square is log2 L shuffles, and a lane's two
 // 16-byte pieces are rotation partners.
 #include "common.cuh"
+#include "ptx.cuh"
 
 namespace decik {
 namespace headrope {
@@ -188,6 +189,7 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(const Args p, int w_dtype
   const int64_t t = static_cast<int64_t>(blockIdx.x) * (kThreads / L) + threadIdx.x / L;
   const bool ok = t < p.n_tok && l.active;
   const int h0 = blockIdx.y * per_group, h1 = h0 + per_group < p.hq + p.hk ? h0 + per_group : p.hq + p.hk;
+  const float inv_d = 1.f / static_cast<float>(p.D);
   float cs[AXES ? 8 : 16], sn[AXES ? 8 : 16];
   load_angles<AXES>(p, l, ok, t, cs, sn);
 #pragma unroll 1
@@ -228,7 +230,7 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(const Args p, int w_dtype
           float ss = 0.f;
 #pragma unroll
           for (int i = 0; i < 16; ++i) ss += x[i] * x[i];
-          r = rsqrtf(row_sum<L>(ss) / p.D + p.eps);
+          r = rsqrtf(row_sum<L>(ss) * inv_d + p.eps);
 #pragma unroll
           for (int i = 0; i < 16; ++i) x[i] *= r;
         }
@@ -246,94 +248,233 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(const Args p, int w_dtype
   }
 }
 
-// The backward with norms. A CTA walks over tiles of 128 / L tokens; a head's row is read while the one
-// before is computed. The weight gradients are summed in fp32: a lane's own rows (the queries' in
-// registers, the keys', which are fewer, in a slot of its own in shared memory), then the CTA's lanes
-// that hold the same values, then the CTAs in a kernel of their own, all in a fixed order.
+// Pairs of fp32 values in one register pair and instruction (the packed arithmetic of sm_100; each half
+// rounds as the single instruction does).
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 pack2f(float x, float y) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpack2f(f2 v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+  f2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+  f2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float sum2(f2 v) {
+  float x, y;
+  unpack2f(v, x, y);
+  return x + y;
+}
+// 8 16-bit values as 4 pairs, and back
+template <typename T>
+__device__ __forceinline__ void unpack_f2(const uint4& v, f2* x) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = pack2f(Dt<T>::lo_f(w[i]), Dt<T>::hi_f(w[i]));
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack_f2(const f2* x) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float a, b;
+    unpack2f(x[i], a, b);
+    w[i] = Dt<T>::pack2(a, b);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// The backward with norms. The rows (tile of 32 / L tokens, head) in tile order are shared out evenly over
+// the warps, each a contiguous range: a warp's lanes keep a tile's angles while its heads last. A row's
+// bytes (gradient, input) are on their way kDepth - 1 rows ahead through cp.async into slots of the
+// lane's own, across heads and tiles. The weight gradients are summed in fp32: a lane's own rows in
+// registers (kept in a slot in shared memory while the warp is at the other part, queries or keys),
+// then the CTA's lanes that hold the same values, then the CTAs in a kernel of their own, all in a
+// fixed order.
+constexpr int kDepth = 4, kSlot = 20;  // kSlot: floats of a lane's slot, 16 and padding against bank conflicts
+
+template <int L, bool LORA>
+constexpr int bwd_smem() {
+  return kThreads * kDepth * (LORA ? 6 : 4) * 16 + (2 * kThreads + 2 * L) * kSlot * 4;
+}
+
 template <typename T, int L, bool AXES, bool LORA>
-__global__ void __launch_bounds__(kThreads) norm_bwd_kernel(const Args p, int w_dtype, int64_t n_tiles) {
-  __shared__ float red[2][kThreads][17];
-  __shared__ float ws[2][16][L];  // weights of lane c: ws[part][i][c]
-  const int c = threadIdx.x % L;
+__global__ void __launch_bounds__(kThreads, LORA ? 3 : 4) norm_bwd_kernel(const Args p, int w_dtype, int64_t n_rows, int64_t per_warp) {
+  constexpr int P = LORA ? 6 : 4, TOK = 32 / L;
+  extern __shared__ __align__(16) unsigned char smem[];
+  float* const slots = reinterpret_cast<float*>(smem + kThreads * kDepth * P * 16);  // [2][kThreads][kSlot]
+  float* const ws = slots + 2 * kThreads * kSlot;                                    // [2][L][kSlot]: weights
+  const int lane = threadIdx.x & 31, c = threadIdx.x % L, heads = p.hq + p.hk;
   const Lane l = lane_of(c, p.D, p.R);
   if (threadIdx.x < 2 * L) {
     float w[16];
     load_weights(threadIdx.x < L ? p.wq : p.wk, w_dtype, l, w);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) ws[threadIdx.x / L][i][c] = w[i];
+    for (int i = 0; i < 16; ++i) ws[threadIdx.x * kSlot + i] = w[i];
   }
-  float dw[16] = {};
 #pragma unroll
-  for (int i = 0; i < 16; ++i) red[1][threadIdx.x][i] = 0.f;
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) slots[(j * kThreads + threadIdx.x) * kSlot + i] = 0.f;
   __syncthreads();
-  for (int64_t tile = blockIdx.x; tile < n_tiles; tile += gridDim.x) {
-    const int64_t t = tile * (kThreads / L) + threadIdx.x / L;
-    const bool ok = t < p.n_tok && l.active;
-    float cs[AXES ? 8 : 16], sn[AXES ? 8 : 16];
-    load_angles<AXES>(p, l, ok, t, cs, sn);
-#pragma unroll 1
-    for (int part = 0; part < 2; ++part) {
-      const decik_tensor3& gr = part ? p.gk : p.gq;
-      const decik_tensor3& in = part ? p.k : p.q;
-      const decik_tensor3_mut& out = part ? p.ok : p.oq;
-      const int heads = part ? p.hk : p.hq;
-      const T* g = static_cast<const T*>(gr.ptr) + t * gr.tok_stride;
-      const T* src = static_cast<const T*>(in.ptr) + t * in.tok_stride;
-      const T* lora = static_cast<const T*>(p.ql.ptr) + t * p.ql.tok_stride;
-      T* dst = static_cast<T*>(out.ptr) + t * out.tok_stride;
-      const bool has_lora = LORA && !part;
-      Raw rg = load_raw(g, l, ok), rx = load_raw(src, l, ok), rl;
-      if constexpr (LORA) rl = load_raw(lora, l, ok && has_lora);
-      for (int h = 0; h < heads; ++h) {
-        float x[16], gv[16], z[16];
-        unpack<T>(rg, gv);
-        unpack<T>(rx, x);
-        if constexpr (LORA) add<T>(rl, x);
-        const bool next = ok && h + 1 < heads;
-        g += gr.head_stride;
-        src += in.head_stride;
-        lora += p.ql.head_stride;
-        rg = load_raw(g, l, next);
-        rx = load_raw(src, l, next);
-        if constexpr (LORA) rl = load_raw(lora, l, next && has_lora);
-        float ss = 0.f, zx = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int hi = AXES ? i : 8 + i;
-          z[i] = gv[i] * cs[i] + gv[8 + i] * sn[hi];
-          z[8 + i] = gv[8 + i] * cs[hi] - gv[i] * sn[i];
+  const int64_t warp = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+  int64_t row = warp * per_warp;
+  const int64_t end = row + per_warp < n_rows ? row + per_warp : n_rows;
+  const float inv_d = 1.f / static_cast<float>(p.D);
+  f2 dw[8] = {};
+  int part = 0;
+  if (row < end) {
+    // the row read next: its token and head and, at a head's start, its addresses
+    int64_t tile = row / heads;
+    int h = static_cast<int>(row - tile * heads);
+    int64_t ft = tile * TOK + lane / L, left = end - row;
+    int fh = h;
+    unsigned char* const ring = smem + threadIdx.x * 16;  // piece q of stage s at (s P + q) kThreads 16
+    auto fetch = [&](int stage) {
+      if (left > 0) {
+        const bool ok = ft < p.n_tok && l.active, k = fh >= p.hq;
+        const int hh = k ? fh - p.hq : fh;
+        const decik_tensor3& gr = k ? p.gk : p.gq;
+        const decik_tensor3& in = k ? p.k : p.q;
+        const T* g = static_cast<const T*>(gr.ptr);
+        const T* x = static_cast<const T*>(in.ptr);
+        if (ok) {
+          g += ft * gr.tok_stride + hh * gr.head_stride;
+          x += ft * in.tok_stride + hh * in.head_stride;
         }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) ss += x[i] * x[i];
-        // (of a row that is not there 0, so that it adds nothing to the sums with eps = 0 either)
-        const float rs = rsqrtf(row_sum<L>(ss) / p.D + p.eps), r = t < p.n_tok ? rs : 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          x[i] *= r;
-          const float d = z[i] * x[i];
-          if (part) red[1][threadIdx.x][i] += d;
-          else dw[i] += d;
-          const float w = ws[part][i][c];
-          zx += d * w;
-          z[i] *= w;
+        const uint32_t dst = ptx::smem_u32(ring) + stage * (P * kThreads * 16);
+        const int lo = ok ? l.lo : 0, hi = ok ? l.hi : 0;
+        ptx::cp_async16(dst, g + lo, ok);
+        ptx::cp_async16(dst + kThreads * 16, g + hi, ok);
+        ptx::cp_async16(dst + 2 * kThreads * 16, x + lo, ok);
+        ptx::cp_async16(dst + 3 * kThreads * 16, x + hi, ok);
+        if constexpr (LORA) {
+          const bool has = ok && !k;
+          const T* y = static_cast<const T*>(p.ql.ptr);
+          if (has) y += ft * p.ql.tok_stride + hh * p.ql.head_stride;
+          ptx::cp_async16(dst + 4 * kThreads * 16, y + (has ? l.lo : 0), has);
+          ptx::cp_async16(dst + 5 * kThreads * 16, y + (has ? l.hi : 0), has);
         }
-        const float mean = row_sum<L>(zx) / p.D;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) z[i] = r * (z[i] - x[i] * mean);
-        if (ok) store(dst, l, z);
-        dst += out.head_stride;
+        --left;
+        if (++fh == heads) fh = 0, ft += TOK;
       }
-    }
-  }
+      ptx::cp_async_commit();
+    };
 #pragma unroll
-  for (int i = 0; i < 16; ++i) red[0][threadIdx.x][i] = dw[i];
+    for (int s = 0; s < kDepth - 1; ++s) fetch(s);
+    int64_t t = tile * TOK + lane / L;
+    bool ok = t < p.n_tok && l.active;
+    // cos of the lane's lo and hi pairs, sin of hi, - sin of lo
+    f2 cl[4], ch[AXES ? 1 : 4], sh[4], nsl[4];
+    auto angles = [&]() {
+      float cs[AXES ? 8 : 16], sn[AXES ? 8 : 16];
+      load_angles<AXES>(p, l, ok, t, cs, sn);
+      constexpr int H = AXES ? 0 : 8;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        cl[i] = pack2f(cs[2 * i], cs[2 * i + 1]);
+        if constexpr (!AXES) ch[i] = pack2f(cs[H + 2 * i], cs[H + 2 * i + 1]);
+        sh[i] = pack2f(sn[H + 2 * i], sn[H + 2 * i + 1]);
+        nsl[i] = pack2f(-sn[2 * i], -sn[2 * i + 1]);
+      }
+    };
+    auto swap = [&](int to) {  // the sums of one part to their slot, those of the other from theirs
+      f2* const a = reinterpret_cast<f2*>(slots + (part * kThreads + threadIdx.x) * kSlot);
+      const f2* const b = reinterpret_cast<const f2*>(slots + (to * kThreads + threadIdx.x) * kSlot);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        a[i] = dw[i];
+        dw[i] = b[i];
+      }
+      part = to;
+    };
+    angles();
+    for (int stage = 0; row < end; ++row) {
+      ptx::cp_async_wait<kDepth - 2>();
+      __syncwarp();  // keeps the reads below behind the wait
+      fetch(stage == 0 ? kDepth - 1 : stage - 1);
+      if ((h >= p.hq) != (part == 1)) swap(part ^ 1);
+      const unsigned char* const got = ring + stage * (P * kThreads * 16);
+      f2 x[8], z[8];
+      {
+        f2 g[8];
+        unpack_f2<T>(*reinterpret_cast<const uint4*>(got), g);
+        unpack_f2<T>(*reinterpret_cast<const uint4*>(got + kThreads * 16), g + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          z[i] = fma2(g[i], cl[i], mul2(g[4 + i], sh[i]));
+          z[4 + i] = fma2(g[4 + i], AXES ? cl[i] : ch[AXES ? 0 : i], mul2(g[i], nsl[i]));
+        }
+      }
+      unpack_f2<T>(*reinterpret_cast<const uint4*>(got + 2 * kThreads * 16), x);
+      unpack_f2<T>(*reinterpret_cast<const uint4*>(got + 3 * kThreads * 16), x + 4);
+      if constexpr (LORA) {
+        f2 y[8];
+        unpack_f2<T>(*reinterpret_cast<const uint4*>(got + 4 * kThreads * 16), y);
+        unpack_f2<T>(*reinterpret_cast<const uint4*>(got + 5 * kThreads * 16), y + 4);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = add2(x[i], y[i]);
+      }
+      f2 ss = mul2(x[0], x[0]);
+#pragma unroll
+      for (int i = 1; i < 8; ++i) ss = fma2(x[i], x[i], ss);
+      // (of a row that is not there 0, so that it adds nothing to the sums with eps = 0 either)
+      const float rs = rsqrtf(row_sum<L>(sum2(ss)) * inv_d + p.eps), r = t < p.n_tok ? rs : 0.f;
+      const f2 rr = pack2f(r, r);
+      f2 zx = 0ull;  // two zeros
+      const ulonglong2* const w = reinterpret_cast<const ulonglong2*>(ws + (part * L + c) * kSlot);
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        const ulonglong2 wv = w[i / 2];
+        x[i] = mul2(x[i], rr);
+        x[i + 1] = mul2(x[i + 1], rr);
+        const f2 d0 = mul2(z[i], x[i]), d1 = mul2(z[i + 1], x[i + 1]);
+        dw[i] = add2(dw[i], d0);
+        dw[i + 1] = add2(dw[i + 1], d1);
+        zx = fma2(d0, wv.x, zx);
+        zx = fma2(d1, wv.y, zx);
+        z[i] = mul2(z[i], wv.x);
+        z[i + 1] = mul2(z[i + 1], wv.y);
+      }
+      const float mean = -row_sum<L>(sum2(zx)) * inv_d;
+      const f2 mm = pack2f(mean, mean);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) z[i] = mul2(rr, fma2(x[i], mm, z[i]));
+      if (ok) {
+        const decik_tensor3_mut& out = part ? p.ok : p.oq;
+        T* const dst = static_cast<T*>(out.ptr) + t * out.tok_stride + (part ? h - p.hq : h) * out.head_stride;
+        stg16(dst + l.lo, pack_f2<T>(z));
+        stg16(dst + l.hi, pack_f2<T>(z + 4));
+      }
+      if (++h == heads) {
+        h = 0;
+        t += TOK;
+        ok = t < p.n_tok && l.active;
+        if (row + 1 < end) angles();
+      }
+      stage = stage + 1 == kDepth ? 0 : stage + 1;
+    }
+    swap(part ^ 1);  // the last sums to their slot
+  }
   __syncthreads();
   for (int j = threadIdx.x; j < 2 * 16 * L; j += kThreads) {  // value i of lane k over the CTA's rows
-    const int part = j / (16 * L), k = j / 16 % L, i = j % 16;
+    const int q = j / (16 * L), k = j / 16 % L, i = j % 16;
     const Lane o = lane_of(k, p.D, p.R);
     float s = 0.f;
-    for (int n = k; n < kThreads; n += L) s += red[part][n][i];
-    if (o.active) p.part[(2 * static_cast<int64_t>(blockIdx.x) + part) * p.D + (i < 8 ? o.lo + i : o.hi + i - 8)] = s;
+    for (int n = k; n < kThreads; n += L) s += slots[(q * kThreads + n) * kSlot + i];
+    if (o.active) p.part[(2 * static_cast<int64_t>(blockIdx.x) + q) * p.D + (i < 8 ? o.lo + i : o.hi + i - 8)] = s;
   }
 }
 
@@ -377,16 +518,29 @@ int launch_fwd_l(const Args& p, bool norm, bool axes, int w_dtype, float sign, c
   return check_launch("head_rope_fwd");
 }
 
+template <typename T, int L, bool AXES, bool LORA>
+int launch_bwd_k(const Args& p, int w_dtype, int* n_part, cudaStream_t s) {
+  static std::atomic<unsigned long long> done{0};
+  auto kernel = norm_bwd_kernel<T, L, AXES, LORA>;
+  if (int rc = ensure_dyn_smem(kernel, bwd_smem<L, LORA>(), done, "head_rope_bwd")) return rc;
+  const int64_t rows = (p.n_tok + 32 / L - 1) / (32 / L) * (p.hq + p.hk);
+  int64_t ctas = static_cast<int64_t>(sm_count()) * (LORA ? 3 : 4);  // all that run at once
+  if (ctas > kMaxPart) ctas = kMaxPart;
+  const int64_t warps = ctas * (kThreads / 32), per_warp = (rows + warps - 1) / warps;
+  const int64_t used = (rows + per_warp - 1) / per_warp;
+  const int grid = static_cast<int>((used + kThreads / 32 - 1) / (kThreads / 32));
+  *n_part = grid;
+  kernel<<<grid, kThreads, bwd_smem<L, LORA>(), s>>>(p, w_dtype, rows, per_warp);
+  return check_launch("head_rope_bwd");
+}
+
 template <typename T, int L>
 int launch_bwd_l(const Args& p, bool axes, int w_dtype, int* n_part, cudaStream_t s) {
-  const int64_t tiles = (p.n_tok + kThreads / L - 1) / (kThreads / L), cap = static_cast<int64_t>(sm_count()) * 4;
-  const int grid = static_cast<int>(tiles < cap ? tiles : cap < kMaxPart ? cap : kMaxPart);
-  *n_part = grid;
-  auto go = [&](auto kernel) { kernel<<<grid, kThreads, 0, s>>>(p, w_dtype, tiles); };
   const bool lora = p.ql.ptr != nullptr;
-  if (axes) lora ? go(norm_bwd_kernel<T, L, true, true>) : go(norm_bwd_kernel<T, L, true, false>);
-  else lora ? go(norm_bwd_kernel<T, L, false, true>) : go(norm_bwd_kernel<T, L, false, false>);
-  return check_launch("head_rope_bwd");
+  if (axes) return lora ? launch_bwd_k<T, L, true, true>(p, w_dtype, n_part, s)
+                        : launch_bwd_k<T, L, true, false>(p, w_dtype, n_part, s);
+  return lora ? launch_bwd_k<T, L, false, true>(p, w_dtype, n_part, s)
+              : launch_bwd_k<T, L, false, false>(p, w_dtype, n_part, s);
 }
 
 template <typename T>
