@@ -329,53 +329,62 @@ __global__ void __launch_bounds__(kThreads, LORA ? 3 : 4) norm_bwd_kernel(const 
 #pragma unroll
     for (int i = 0; i < 16; ++i) slots[(j * kThreads + threadIdx.x) * kSlot + i] = 0.f;
   __syncthreads();
-  const int64_t warp = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
-  int64_t row = warp * per_warp;
-  const int64_t end = row + per_warp < n_rows ? row + per_warp : n_rows;
+  // the warp's number broadcast, so that the row's state below lives in uniform registers
+  const int64_t warp = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+  const int64_t row0 = warp * per_warp;
+  int left = static_cast<int>(n_rows - row0 < per_warp ? n_rows - row0 : per_warp);
   const float inv_d = 1.f / static_cast<float>(p.D);
   f2 dw[8] = {};
   int part = 0;
-  if (row < end) {
-    // the row read next: its token and head and, at a head's start, its addresses
-    int64_t tile = row / heads;
-    int h = static_cast<int>(row - tile * heads);
-    int64_t ft = tile * TOK + lane / L, left = end - row;
-    int fh = h;
-    unsigned char* const ring = smem + threadIdx.x * 16;  // piece q of stage s at (s P + q) kThreads 16
+  if (left > 0) {
+    // The row read next: its tile, head and running addresses, set anew where a part begins. A lane
+    // without a value of its own (beyond the tokens, or D) reads nothing, from an address that is there.
+    const int tile0 = static_cast<int>(row0 / heads), n_tok = static_cast<int>(p.n_tok);
+    const int off = l.active ? l.lo : 0, up = l.active ? l.hi - l.lo : 0;
+    int h = static_cast<int>(row0 - static_cast<int64_t>(tile0) * heads);
+    int fh = h, to_read = left, ft = tile0 * TOK + lane / L;
+    const T *g, *x, *y = nullptr;
+    const uint32_t ring_at = ptx::smem_u32(smem + threadIdx.x * 16);  // piece q of stage s at (s P + q) kThreads 16
+    auto seek = [&]() {
+      const int64_t t = ft < n_tok ? ft : n_tok - 1;
+      const bool k = fh >= p.hq;
+      const int hh = k ? fh - p.hq : fh;
+      const decik_tensor3& gr = k ? p.gk : p.gq;
+      const decik_tensor3& in = k ? p.k : p.q;
+      g = static_cast<const T*>(gr.ptr) + t * gr.tok_stride + hh * gr.head_stride + off;
+      x = static_cast<const T*>(in.ptr) + t * in.tok_stride + hh * in.head_stride + off;
+      if constexpr (LORA) y = static_cast<const T*>(p.ql.ptr) + t * p.ql.tok_stride + (k ? 0 : hh * p.ql.head_stride) + off;
+    };
+    seek();
     auto fetch = [&](int stage) {
-      if (left > 0) {
-        const bool ok = ft < p.n_tok && l.active, k = fh >= p.hq;
-        const int hh = k ? fh - p.hq : fh;
-        const decik_tensor3& gr = k ? p.gk : p.gq;
-        const decik_tensor3& in = k ? p.k : p.q;
-        const T* g = static_cast<const T*>(gr.ptr);
-        const T* x = static_cast<const T*>(in.ptr);
-        if (ok) {
-          g += ft * gr.tok_stride + hh * gr.head_stride;
-          x += ft * in.tok_stride + hh * in.head_stride;
-        }
-        const uint32_t dst = ptx::smem_u32(ring) + stage * (P * kThreads * 16);
-        const int lo = ok ? l.lo : 0, hi = ok ? l.hi : 0;
-        ptx::cp_async16(dst, g + lo, ok);
-        ptx::cp_async16(dst + kThreads * 16, g + hi, ok);
-        ptx::cp_async16(dst + 2 * kThreads * 16, x + lo, ok);
-        ptx::cp_async16(dst + 3 * kThreads * 16, x + hi, ok);
+      if (to_read > 0) {
+        const uint32_t dst = ring_at + stage * (P * kThreads * 16);
+        const bool there = ft < n_tok && l.active, k = fh >= p.hq;
+        ptx::cp_async16(dst, g, there);
+        ptx::cp_async16(dst + kThreads * 16, g + up, there);
+        ptx::cp_async16(dst + 2 * kThreads * 16, x, there);
+        ptx::cp_async16(dst + 3 * kThreads * 16, x + up, there);
         if constexpr (LORA) {
-          const bool has = ok && !k;
-          const T* y = static_cast<const T*>(p.ql.ptr);
-          if (has) y += ft * p.ql.tok_stride + hh * p.ql.head_stride;
-          ptx::cp_async16(dst + 4 * kThreads * 16, y + (has ? l.lo : 0), has);
-          ptx::cp_async16(dst + 5 * kThreads * 16, y + (has ? l.hi : 0), has);
+          ptx::cp_async16(dst + 4 * kThreads * 16, y, there && !k);
+          ptx::cp_async16(dst + 5 * kThreads * 16, y + up, there && !k);
+          if (!k && fh + 1 < p.hq) y += p.ql.head_stride;
         }
-        --left;
-        if (++fh == heads) fh = 0, ft += TOK;
+        ++fh;
+        --to_read;
+        if (fh == heads) fh = 0, ft += TOK;
+        if (fh == 0 || fh == p.hq) {
+          seek();
+        } else {
+          g += k ? p.gk.head_stride : p.gq.head_stride;
+          x += k ? p.k.head_stride : p.q.head_stride;
+        }
       }
       ptx::cp_async_commit();
     };
 #pragma unroll
     for (int s = 0; s < kDepth - 1; ++s) fetch(s);
-    int64_t t = tile * TOK + lane / L;
-    bool ok = t < p.n_tok && l.active;
+    int t = tile0 * TOK + lane / L;
+    bool ok = t < n_tok && l.active;
     // cos of the lane's lo and hi pairs, sin of hi, - sin of lo
     f2 cl[4], ch[AXES ? 1 : 4], sh[4], nsl[4];
     auto angles = [&]() {
@@ -400,47 +409,53 @@ __global__ void __launch_bounds__(kThreads, LORA ? 3 : 4) norm_bwd_kernel(const 
       }
       part = to;
     };
+    T* dst;  // the result's running address
+    auto aim = [&]() {
+      const decik_tensor3_mut& out = h >= p.hq ? p.ok : p.oq;
+      dst = static_cast<T*>(out.ptr) + t * out.tok_stride + (h >= p.hq ? h - p.hq : h) * out.head_stride + off;
+    };
     angles();
-    for (int stage = 0; row < end; ++row) {
+    aim();
+    for (int stage = 0; left > 0; --left) {
       ptx::cp_async_wait<kDepth - 2>();
       __syncwarp();  // keeps the reads below behind the wait
       fetch(stage == 0 ? kDepth - 1 : stage - 1);
       if ((h >= p.hq) != (part == 1)) swap(part ^ 1);
-      const unsigned char* const got = ring + stage * (P * kThreads * 16);
-      f2 x[8], z[8];
+      const unsigned char* const got = smem + threadIdx.x * 16 + stage * (P * kThreads * 16);
+      f2 v[8], z[8];
       {
-        f2 g[8];
-        unpack_f2<T>(*reinterpret_cast<const uint4*>(got), g);
-        unpack_f2<T>(*reinterpret_cast<const uint4*>(got + kThreads * 16), g + 4);
+        f2 gv[8];
+        unpack_f2<T>(*reinterpret_cast<const uint4*>(got), gv);
+        unpack_f2<T>(*reinterpret_cast<const uint4*>(got + kThreads * 16), gv + 4);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          z[i] = fma2(g[i], cl[i], mul2(g[4 + i], sh[i]));
-          z[4 + i] = fma2(g[4 + i], AXES ? cl[i] : ch[AXES ? 0 : i], mul2(g[i], nsl[i]));
+          z[i] = fma2(gv[i], cl[i], mul2(gv[4 + i], sh[i]));
+          z[4 + i] = fma2(gv[4 + i], AXES ? cl[i] : ch[AXES ? 0 : i], mul2(gv[i], nsl[i]));
         }
       }
-      unpack_f2<T>(*reinterpret_cast<const uint4*>(got + 2 * kThreads * 16), x);
-      unpack_f2<T>(*reinterpret_cast<const uint4*>(got + 3 * kThreads * 16), x + 4);
+      unpack_f2<T>(*reinterpret_cast<const uint4*>(got + 2 * kThreads * 16), v);
+      unpack_f2<T>(*reinterpret_cast<const uint4*>(got + 3 * kThreads * 16), v + 4);
       if constexpr (LORA) {
-        f2 y[8];
-        unpack_f2<T>(*reinterpret_cast<const uint4*>(got + 4 * kThreads * 16), y);
-        unpack_f2<T>(*reinterpret_cast<const uint4*>(got + 5 * kThreads * 16), y + 4);
+        f2 yv[8];
+        unpack_f2<T>(*reinterpret_cast<const uint4*>(got + 4 * kThreads * 16), yv);
+        unpack_f2<T>(*reinterpret_cast<const uint4*>(got + 5 * kThreads * 16), yv + 4);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = add2(x[i], y[i]);
+        for (int i = 0; i < 8; ++i) v[i] = add2(v[i], yv[i]);
       }
-      f2 ss = mul2(x[0], x[0]);
+      f2 ss = mul2(v[0], v[0]);
 #pragma unroll
-      for (int i = 1; i < 8; ++i) ss = fma2(x[i], x[i], ss);
+      for (int i = 1; i < 8; ++i) ss = fma2(v[i], v[i], ss);
       // (of a row that is not there 0, so that it adds nothing to the sums with eps = 0 either)
-      const float rs = rsqrtf(row_sum<L>(sum2(ss)) * inv_d + p.eps), r = t < p.n_tok ? rs : 0.f;
+      const float rs = rsqrtf(row_sum<L>(sum2(ss)) * inv_d + p.eps), r = t < n_tok ? rs : 0.f;
       const f2 rr = pack2f(r, r);
       f2 zx = 0ull;  // two zeros
       const ulonglong2* const w = reinterpret_cast<const ulonglong2*>(ws + (part * L + c) * kSlot);
 #pragma unroll
       for (int i = 0; i < 8; i += 2) {
         const ulonglong2 wv = w[i / 2];
-        x[i] = mul2(x[i], rr);
-        x[i + 1] = mul2(x[i + 1], rr);
-        const f2 d0 = mul2(z[i], x[i]), d1 = mul2(z[i + 1], x[i + 1]);
+        v[i] = mul2(v[i], rr);
+        v[i + 1] = mul2(v[i + 1], rr);
+        const f2 d0 = mul2(z[i], v[i]), d1 = mul2(z[i + 1], v[i + 1]);
         dw[i] = add2(dw[i], d0);
         dw[i + 1] = add2(dw[i + 1], d1);
         zx = fma2(d0, wv.x, zx);
@@ -451,19 +466,19 @@ __global__ void __launch_bounds__(kThreads, LORA ? 3 : 4) norm_bwd_kernel(const 
       const float mean = -row_sum<L>(sum2(zx)) * inv_d;
       const f2 mm = pack2f(mean, mean);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) z[i] = mul2(rr, fma2(x[i], mm, z[i]));
+      for (int i = 0; i < 8; ++i) z[i] = mul2(rr, fma2(v[i], mm, z[i]));
       if (ok) {
-        const decik_tensor3_mut& out = part ? p.ok : p.oq;
-        T* const dst = static_cast<T*>(out.ptr) + t * out.tok_stride + (part ? h - p.hq : h) * out.head_stride;
-        stg16(dst + l.lo, pack_f2<T>(z));
-        stg16(dst + l.hi, pack_f2<T>(z + 4));
+        stg16(dst, pack_f2<T>(z));
+        stg16(dst + up, pack_f2<T>(z + 4));
       }
       if (++h == heads) {
         h = 0;
         t += TOK;
-        ok = t < p.n_tok && l.active;
-        if (row + 1 < end) angles();
+        ok = t < n_tok && l.active;
+        if (left > 1) angles();
       }
+      if (h == 0 || h == p.hq) aim();
+      else dst += part ? p.ok.head_stride : p.oq.head_stride;
       stage = stage + 1 == kDepth ? 0 : stage + 1;
     }
     swap(part ^ 1);  // the last sums to their slot
