@@ -303,7 +303,7 @@ __device__ __forceinline__ uint4 pack_f2(const f2* x) {
 // registers (kept in a slot in shared memory while the warp is at the other part, queries or keys),
 // then the CTA's lanes that hold the same values, then the CTAs in a kernel of their own, all in a
 // fixed order.
-constexpr int kDepth = 4, kSlot = 20;  // kSlot: floats of a lane's slot, 16 and padding against bank conflicts
+constexpr int kDepth = 3, kSlot = 20;  // kSlot: floats of a lane's slot, 16 and padding against bank conflicts
 
 template <int L, bool LORA>
 constexpr int bwd_smem() {
@@ -442,13 +442,16 @@ __global__ void __launch_bounds__(kThreads, LORA ? 3 : 4) norm_bwd_kernel(const 
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = add2(v[i], yv[i]);
       }
-      f2 ss = mul2(v[0], v[0]);
+      f2 ss0 = mul2(v[0], v[0]), ss1 = mul2(v[1], v[1]);
 #pragma unroll
-      for (int i = 1; i < 8; ++i) ss = fma2(v[i], v[i], ss);
+      for (int i = 2; i < 8; i += 2) {
+        ss0 = fma2(v[i], v[i], ss0);
+        ss1 = fma2(v[i + 1], v[i + 1], ss1);
+      }
       // (of a row that is not there 0, so that it adds nothing to the sums with eps = 0 either)
-      const float rs = rsqrtf(row_sum<L>(sum2(ss)) * inv_d + p.eps), r = t < n_tok ? rs : 0.f;
+      const float rs = rsqrtf(row_sum<L>(sum2(add2(ss0, ss1))) * inv_d + p.eps), r = t < n_tok ? rs : 0.f;
       const f2 rr = pack2f(r, r);
-      f2 zx = 0ull;  // two zeros
+      f2 zx0 = 0ull, zx1 = 0ull;  // two zeros each
       const ulonglong2* const w = reinterpret_cast<const ulonglong2*>(ws + (part * L + c) * kSlot);
 #pragma unroll
       for (int i = 0; i < 8; i += 2) {
@@ -458,12 +461,12 @@ __global__ void __launch_bounds__(kThreads, LORA ? 3 : 4) norm_bwd_kernel(const 
         const f2 d0 = mul2(z[i], v[i]), d1 = mul2(z[i + 1], v[i + 1]);
         dw[i] = add2(dw[i], d0);
         dw[i + 1] = add2(dw[i + 1], d1);
-        zx = fma2(d0, wv.x, zx);
-        zx = fma2(d1, wv.y, zx);
+        zx0 = fma2(d0, wv.x, zx0);
+        zx1 = fma2(d1, wv.y, zx1);
         z[i] = mul2(z[i], wv.x);
         z[i + 1] = mul2(z[i + 1], wv.y);
       }
-      const float mean = -row_sum<L>(sum2(zx)) * inv_d;
+      const float mean = -row_sum<L>(sum2(add2(zx0, zx1))) * inv_d;
       const f2 mm = pack2f(mean, mean);
 #pragma unroll
       for (int i = 0; i < 8; ++i) z[i] = mul2(rr, fma2(v[i], mm, z[i]));
