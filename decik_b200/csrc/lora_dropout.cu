@@ -39,6 +39,29 @@ __device__ __forceinline__ void mask8(const uint4& w, const uint4& v, uint32_t l
   m[3] = mask_pair(v.w, keep_lo(w.w, limit), keep_hi(w.w, limit));
 }
 
+// fp32 blocks of 32 columns in shared memory: row r's 16-byte piece q (of 8) at r * 128 + 16 (q ^ r % 8). They
+// are copied a whole row by 8 lanes (whole 32-byte sectors; a lane fetching its own 32 bytes in two
+// pieces asked L2 for every sector twice) and read back as two pieces 2 c, 2 c + 1 of row g without bank
+// conflicts.
+__device__ __forceinline__ uint32_t block_at(int r, int q) { return r * 128 + ((q ^ (r & 7)) * 16); }
+__device__ __forceinline__ void block_read(const unsigned char* p, int r, int c, float (&f)[8]) {
+  const float4 a = *reinterpret_cast<const float4*>(p + block_at(r, 2 * c));
+  const float4 b = *reinterpret_cast<const float4*>(p + block_at(r, 2 * c + 1));
+  f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+}
+
+// 8 fp32 values to global memory: one 32-byte store where the rows allow it
+__device__ __forceinline__ void store32(float* p, const float (&f)[8], bool whole) {
+  if (whole) {
+    asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(f[0]), "f"(f[1]), "f"(f[2]),
+                 "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7])
+                 : "memory");
+  } else {
+    reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+  }
+}
+
 // transpose of an 8 x 8 matrix of 16-bit values held by a warp (lane 4 i + c: row i, columns 2 c, 2 c + 1)
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t r;
@@ -55,8 +78,8 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
 // the order of a sum's terms is free, an operand fragment of mma.sync m16n8k16 without any exchange:
 // the instruction's columns 2 c, 2 c + 1 and 2 c + 8, 2 c + 9 of step s are the lane's pairs 2 s and
 // 2 s + 1. lora_A's rows, read the same way (16 bytes of row g), are the other operand.
-// The next block's bytes are on their way through cp.async while one is computed: a lane reads back
-// only what it copied itself, so shared memory serves as its registers and no barrier is needed.
+// The next block's bytes are on their way through cp.async, into the warp's own ring, while one is
+// computed.
 template <typename X, typename T, int NB, int NTB, int MT>
 struct DownTile {
   static constexpr int kXPieces = sizeof(X) / 2;                       // 16-byte pieces of 8 columns
@@ -89,55 +112,55 @@ down_kernel(const X* __restrict__ x, int64_t ldx, const T* __restrict__ a, int64
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[m][n][e] = 0.f;
-  unsigned char* const ring = smem + warp * (2 * Tile::kStage) + lane * 16;
+  unsigned char* const ring = smem + warp * (2 * Tile::kStage);  // x, then A: a lane's own piece n at 512 n + 16 lane
+  constexpr int kXBytes = 2 * MT * XP * 512;
   const int rows = n_tok - t0 < 16 * MT ? static_cast<int>(n_tok - t0) : 16 * MT;
-  // the lane's pieces of the block with its columns at k (zeros outside the matrix)
-  const X* const xp = x + (t0 + g) * ldx;
-  const T* const ap = a + static_cast<int64_t>(g) * lda;
-  auto issue = [&](int stage, int k) {
+  // the pieces of the block with its columns at k0 (zeros outside the matrix)
+  const int xr = XP == 2 ? lane >> 3 : g, xc = XP == 2 ? 4 * (lane & 7) : 8 * c;  // the lane's row and column in a copy
+  const X* const xp = x + (t0 + xr) * ldx + xc;
+  const T* const ap = a + static_cast<int64_t>(g) * lda + 8 * c;
+  auto issue = [&](int stage, int k0) {
     const uint32_t dst = ptx::smem_u32(ring) + stage * Tile::kStage;
-    const bool in = k < width;
+    const bool in = k0 + xc < width;
 #pragma unroll
-    for (int i = 0; i < 2 * MT; ++i) {
-      const bool ok = in && 8 * i + g < rows;
-      const X* src = ok ? xp + 8 * i * ldx + k : x;
-#pragma unroll
-      for (int j = 0; j < XP; ++j)
-        ptx::cp_async16(dst + (i * XP + j) * 512, reinterpret_cast<const char*>(src) + 16 * j, ok);
+    for (int i = 0; i < 2 * MT * XP; ++i) {
+      const int r = (XP == 2 ? 4 : 8) * i + xr;
+      const bool ok = in && r < rows;
+      ptx::cp_async16(dst + (XP == 2 ? block_at(r, lane & 7) : i * 512 + lane * 16),
+                      ok ? xp + (XP == 2 ? 4 : 8) * i * ldx + k0 : x, ok);
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int r = 8 * (n % NTB);
-      const bool ok = in && r < rank;
-      ptx::cp_async16(dst + (2 * MT * XP + n) * 512, ok ? ap + (n / NTB * rank + r) * lda + k : a, ok);
+      const bool ok = k0 + 8 * c < width && r < rank;
+      ptx::cp_async16(dst + kXBytes + n * 512 + lane * 16, ok ? ap + (n / NTB * rank + r) * lda + k0 : a, ok);
     }
   };
   int stage = 0;
   const int step = 32 * WARPS;
   const unsigned long long group0 = static_cast<unsigned long long>(t0 + g) * (width / 8);
-  if (32 * warp < width) issue(0, 32 * warp + 8 * c);
+  if (32 * warp < width) issue(0, 32 * warp);
   ptx::cp_async_commit();
   for (int k = 32 * warp + 8 * c; k - 8 * c < width; k += step, stage ^= 1) {
     __syncwarp();  // the other stage has been read
-    if (k - 8 * c + step < width) issue(stage ^ 1, k + step);
+    if (k - 8 * c + step < width) issue(stage ^ 1, k - 8 * c + step);
     ptx::cp_async_commit();
     ptx::cp_async_wait<1>();
     __syncwarp();
-    const uint4* got = reinterpret_cast<const uint4*>(ring + stage * Tile::kStage);
+    const unsigned char* const got = ring + stage * Tile::kStage;
     uint4 av[NT];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) av[n] = got[(2 * MT * XP + n) * 32];
+    for (int n = 0; n < NT; ++n) av[n] = *reinterpret_cast<const uint4*>(got + kXBytes + n * 512 + lane * 16);
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       uint4 xv[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint4* p = got + (2 * m + h) * XP * 32;
         if constexpr (XP == 1) {
-          xv[h] = p[0];
+          xv[h] = *reinterpret_cast<const uint4*>(got + (2 * m + h) * 512 + lane * 16);
         } else {
-          const float4 lo = *reinterpret_cast<const float4*>(p), hi = *reinterpret_cast<const float4*>(p + 32);
-          const float f[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+          float f[8];
+          block_read(got, 16 * m + 8 * h + g, c, f);
           xv[h] = pack8<T>(f);
         }
         if (x16 != nullptr && k < width && 16 * m + 8 * h + g < rows)
@@ -252,7 +275,9 @@ bwd_kernel(const T* __restrict__ du, int64_t ld_du, const T* __restrict__ x16, i
   const uint32_t ring_at = ptx::smem_u32(ring);
   // running addresses: of the tile issued next, and of dx and the generator's group of the one computed
   const T* xp = x16 + (first + g) * ldx + k;
-  const float* addp = addend != nullptr ? addend + (first + g) * ld_add + k : nullptr;
+  const int ar = lane >> 3, ac = 32 * cb + 4 * (lane & 7);  // the lane's row and column in a copy of the addend
+  const float* addp = addend != nullptr ? addend + (first + ar) * ld_add + ac : nullptr;
+  const bool whole = ld_dx % 8 == 0 && (reinterpret_cast<uintptr_t>(dx) & 31) == 0;
   float* dxp = dx + (first + g) * ld_dx + k;
   const T* dup[NB * KR];
   uint32_t du_dst[NB * KR];
@@ -270,10 +295,14 @@ bwd_kernel(const T* __restrict__ du, int64_t ld_du, const T* __restrict__ x16, i
     for (int h = 0; h < 2; ++h) {
       const bool ok = in && i0 + 8 * h + g < n;
       ptx::cp_async16(dst + h * 512 + lane * 16, ok ? xp + 8 * h * ldx : x16, ok);
-      if (addend == nullptr) continue;
-      const float* src = ok ? addp + 8 * h * ld_add : addend;
-      ptx::cp_async16(dst + (2 + 2 * h) * 512 + lane * 16, src, ok);
-      ptx::cp_async16(dst + (3 + 2 * h) * 512 + lane * 16, ok ? src + 4 : src, ok);
+    }
+    if (addend != nullptr) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = 4 * i + ar;
+        const bool ok = ac < width && r < n - i0;
+        ptx::cp_async16(dst + 2 * 512 + block_at(r, lane & 7), ok ? addp + 4 * i * ld_add : addend, ok);
+      }
     }
 #pragma unroll
     for (int q = 0; q < NB * KR; ++q) {
@@ -305,12 +334,7 @@ bwd_kernel(const T* __restrict__ du, int64_t ld_du, const T* __restrict__ x16, i
       xv[h] = *reinterpret_cast<const uint4*>(got + h * 512 + lane * 16);
 #pragma unroll
       for (int i = 0; i < 8; ++i) out[h][i] = 0.f;
-      if (addend != nullptr) {
-        const float4 lo = *reinterpret_cast<const float4*>(got + (2 + 2 * h) * 512 + lane * 16);
-        const float4 hi = *reinterpret_cast<const float4*>(got + (3 + 2 * h) * 512 + lane * 16);
-        out[h][0] = lo.x, out[h][1] = lo.y, out[h][2] = lo.z, out[h][3] = lo.w;
-        out[h][4] = hi.x, out[h][5] = hi.y, out[h][6] = hi.z, out[h][7] = hi.w;
-      }
+      if (addend != nullptr) block_read(got + 2 * 512, 8 * h + g, c, out[h]);
     }
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
@@ -356,11 +380,7 @@ bwd_kernel(const T* __restrict__ du, int64_t ld_du, const T* __restrict__ x16, i
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h)
-      if (in && i0 + 8 * h + g < n) {
-        float4* o = reinterpret_cast<float4*>(dxp + 8 * h * ld_dx);
-        o[0] = make_float4(out[h][0], out[h][1], out[h][2], out[h][3]);
-        o[1] = make_float4(out[h][4], out[h][5], out[h][6], out[h][7]);
-      }
+      if (in && i0 + 8 * h + g < n) store32(dxp + 8 * h * ld_dx, out[h], whole);
     stage = stage + 1 == kBwdStages ? 0 : stage + 1;
   }
   if (!in) return;
