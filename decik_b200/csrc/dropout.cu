@@ -49,7 +49,8 @@ template <typename X, typename O, bool RES, bool VEC>
 __global__ void __launch_bounds__(256)
 dropout_kernel(const X* x, const O* residual, O* out, int64_t n, uint32_t cut, float scale,
                const int64_t* __restrict__ rng, int64_t stream_id) {
-  const philox::Key key = philox::make_key(rng, stream_id);
+  const philox::Key key = philox::make_key(rng);
+  const philox::Stream ctr = philox::make_stream(rng, stream_id);
   const int64_t groups = (n + 7) / 8, whole = VEC ? n / 8 : 0;
   const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
   int64_t g = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
@@ -67,7 +68,7 @@ dropout_kernel(const X* x, const O* residual, O* out, int64_t n, uint32_t cut, f
       for (int u = 0; u < kUnroll; ++u) {
         const int64_t i = g + u * stride;
         if (i >= whole) break;
-        const uint4 w = philox::words(key, static_cast<unsigned long long>(i));
+        const uint4 w = philox::words(key, ctr, static_cast<unsigned long long>(i));
         float f[8], o[8] = {};
         xv[u].values(f);
         if constexpr (RES) rv[u].values(o);
@@ -82,7 +83,7 @@ dropout_kernel(const X* x, const O* residual, O* out, int64_t n, uint32_t cut, f
     g = whole + static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;  // the last group, if it is not whole
   }
   for (; g < groups; g += stride) {
-    const uint4 w = philox::words(key, static_cast<unsigned long long>(g));
+    const uint4 w = philox::words(key, ctr, static_cast<unsigned long long>(g));
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int64_t i = 8 * g + j;

@@ -15,28 +15,46 @@ namespace {
 
 constexpr int kMaxRank = 64;  // rows of A over all branches
 
-// per branch: a lane of the generator, in the high half of a word, is kept iff the word >= limit; a
-// scale of 0 means that nothing is kept (p = 1)
+// per branch: a 16-bit lane of the generator is kept iff it is >= cut; a scale of 0 means that nothing is
+// kept (p = 1, whose cut does not fit the lane)
 struct Drop {
-  uint32_t limit[2];
+  uint32_t cut[2];    // in both halves of the word
   float scale[2];
+  // 0xffff, 65536 and -1, as arguments: products with values that the compiler does not know stay products,
+  // on the FMA pipe, where constants would become shifts and additions on the ALU pipe, the busiest here
+  uint32_t ones, shift, minus;
 };
 
-// The kept values of a pair v of 16-bit values under one word of the generator. Predicated ands on two
-// compares: the shift runs on the FMA pipe, which leaves four instructions for the ALU pipe, the one
-// these kernels keep busiest.
-__device__ __forceinline__ bool keep_lo(uint32_t w, uint32_t limit) { return w * 65536u >= limit; }
-__device__ __forceinline__ bool keep_hi(uint32_t w, uint32_t limit) { return w >= limit; }
-__device__ __forceinline__ uint32_t mask_pair(uint32_t v, bool lo, bool hi) {
-  if (!lo) v &= 0xFFFF0000u;
-  if (!hi) v &= 0x0000FFFFu;
-  return v;
+// The kept values of a pair v of 16-bit values under one word of the generator, in 3 instructions of the ALU
+// pipe and 2 products: max(w, cut) - w is 0 in the halves that are kept (no borrow crosses them), min with
+// 1 makes that a bit, times 0xffff a mask.
+__device__ __forceinline__ uint32_t mask_pair(uint32_t w, uint32_t v, uint32_t cut, const Drop& k) {
+  uint32_t m, d;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(m) : "r"(w), "r"(cut));
+  asm("min.u16x2 %0, %1, %2;" : "=r"(d) : "r"(w * k.minus + m), "r"(0x00010001u));
+  return v & ~(d * k.ones);
 }
-__device__ __forceinline__ void mask8(const uint4& w, const uint4& v, uint32_t limit, uint32_t (&m)[4]) {
-  m[0] = mask_pair(v.x, keep_lo(w.x, limit), keep_hi(w.x, limit));
-  m[1] = mask_pair(v.y, keep_lo(w.y, limit), keep_hi(w.y, limit));
-  m[2] = mask_pair(v.z, keep_lo(w.z, limit), keep_hi(w.z, limit));
-  m[3] = mask_pair(v.w, keep_lo(w.w, limit), keep_hi(w.w, limit));
+__device__ __forceinline__ void mask8(const uint4& w, const uint4& v, uint32_t cut, const Drop& k, uint32_t (&m)[4]) {
+  m[0] = mask_pair(w.x, v.x, cut, k);
+  m[1] = mask_pair(w.y, v.y, cut, k);
+  m[2] = mask_pair(w.z, v.z, cut, k);
+  m[3] = mask_pair(w.w, v.w, cut, k);
+}
+// The same for a pair whose products are wanted too: v masked, and o0, o1 += scale * p0, p1 where kept. One
+// compare serves a value's two uses, as the predicate of an fma and of an and.
+__device__ __forceinline__ uint32_t mask_add_pair(uint32_t w, uint32_t v, uint32_t limit, uint32_t shift, float scale,
+                                                  float p0, float p1, float& o0, float& o1) {
+  asm("{\n\t.reg .pred l, h;\n\t.reg .b32 t;\n\t"
+      "mul.lo.u32 t, %3, %5;\n\t"
+      "setp.ge.u32 l, t, %4;\n\t"
+      "setp.ge.u32 h, %3, %4;\n\t"
+      "@l fma.rn.f32 %1, %6, %7, %1;\n\t"
+      "@h fma.rn.f32 %2, %6, %8, %2;\n\t"
+      "@!l and.b32 %0, %0, 0xffff0000;\n\t"
+      "@!h and.b32 %0, %0, 0x0000ffff;\n\t}"
+      : "+r"(v), "+f"(o0), "+f"(o1)
+      : "r"(w), "r"(limit), "r"(shift), "f"(scale), "f"(p0), "f"(p1));
+  return v;
 }
 
 // fp32 blocks of 32 columns in shared memory: row r's 16-byte piece q (of 8) at r * 128 + 16 (q ^ r % 8). They
@@ -93,7 +111,7 @@ struct DownTile {
 };
 
 template <typename X, typename T, int NB, int NTB, int MT, int WARPS>
-__global__ void __launch_bounds__(32 * WARPS, NB * NTB <= 4 ? 16 / WARPS : 8 / WARPS)
+__global__ void __launch_bounds__(32 * WARPS, NB * NTB <= 4 ? (WARPS == 4 ? 5 : 2) : 8 / WARPS)
 down_kernel(const X* __restrict__ x, int64_t ldx, const T* __restrict__ a, int64_t lda, T* __restrict__ x16,
             int64_t ldx16, T* __restrict__ u, int64_t ldu, int64_t n_tok, int width, int rank, Drop d,
             const int64_t* __restrict__ rng, int64_t stream_id) {
@@ -102,9 +120,10 @@ down_kernel(const X* __restrict__ x, int64_t ldx, const T* __restrict__ a, int64
   extern __shared__ __align__(16) unsigned char smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * (16 * MT);
-  philox::Key key[NB];
+  const philox::Key key = philox::make_key(rng);
+  philox::Stream ctr[NB];
 #pragma unroll
-  for (int b = 0; b < NB; ++b) key[b] = philox::make_key(rng, stream_id + b);
+  for (int b = 0; b < NB; ++b) ctr[b] = philox::make_stream(rng, stream_id + b);
   float acc[MT][NT][4];
 #pragma unroll
   for (int m = 0; m < MT; ++m)
@@ -115,29 +134,30 @@ down_kernel(const X* __restrict__ x, int64_t ldx, const T* __restrict__ a, int64
   unsigned char* const ring = smem + warp * (2 * Tile::kStage);  // x, then A: a lane's own piece n at 512 n + 16 lane
   constexpr int kXBytes = 2 * MT * XP * 512;
   const int rows = n_tok - t0 < 16 * MT ? static_cast<int>(n_tok - t0) : 16 * MT;
-  // the pieces of the block with its columns at k0 (zeros outside the matrix)
-  const int xr = XP == 2 ? lane >> 3 : g, xc = XP == 2 ? 4 * (lane & 7) : 8 * c;  // the lane's row and column in a copy
-  const X* const xp = x + (t0 + xr) * ldx + xc;
-  const T* const ap = a + static_cast<int64_t>(g) * lda + 8 * c;
+  // The pieces of the block with its columns at k0, zeros behind the width. Rows that are not there (of x
+  // behind the last token, of A behind the rank) are others read again: what comes of them is not stored.
+  constexpr int XN = 2 * MT * XP, XR = XP == 2 ? 4 : 8, XE = 16 / sizeof(X);  // a copy's pieces, rows, elements
+  const int xr = XP == 2 ? lane >> 3 : g, xc = XP == 2 ? 4 * (lane & 7) : 8 * c;  // the lane's row and column
+  const X* xp[XN];
+  const T* ap[NT];
+#pragma unroll
+  for (int i = 0; i < XN; ++i) xp[i] = x + (t0 + (XR * i + xr < rows ? XR * i + xr : 0)) * ldx;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) ap[n] = a + static_cast<int64_t>(8 * (n % NTB) < rank ? n / NTB * rank + 8 * (n % NTB) + g : 0) * lda;
   auto issue = [&](int stage, int k0) {
     const uint32_t dst = ptx::smem_u32(ring) + stage * Tile::kStage;
-    const bool in = k0 + xc < width;
+    const bool xin = k0 + xc < width, ain = k0 + 8 * c < width;
+    const int xk = xin ? k0 + xc : width - XE, ak = ain ? k0 + 8 * c : width - 8;
 #pragma unroll
-    for (int i = 0; i < 2 * MT * XP; ++i) {
-      const int r = (XP == 2 ? 4 : 8) * i + xr;
-      const bool ok = in && r < rows;
-      ptx::cp_async16(dst + (XP == 2 ? block_at(r, lane & 7) : i * 512 + lane * 16),
-                      ok ? xp + (XP == 2 ? 4 : 8) * i * ldx + k0 : x, ok);
-    }
+    for (int i = 0; i < XN; ++i)
+      ptx::cp_async16(dst + (XP == 2 ? block_at(XR * i + xr, lane & 7) : i * 512 + lane * 16), xp[i] + xk, xin);
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int r = 8 * (n % NTB);
-      const bool ok = k0 + 8 * c < width && r < rank;
-      ptx::cp_async16(dst + kXBytes + n * 512 + lane * 16, ok ? ap + (n / NTB * rank + r) * lda + k0 : a, ok);
-    }
+    for (int n = 0; n < NT; ++n)
+      ptx::cp_async16(dst + kXBytes + n * 512 + lane * 16, ap[n] + ak, ain);
   };
   int stage = 0;
   const int step = 32 * WARPS;
+  T* const x16p = x16 + (t0 + g) * ldx16;
   const unsigned long long group0 = static_cast<unsigned long long>(t0 + g) * (width / 8);
   if (32 * warp < width) issue(0, 32 * warp);
   ptx::cp_async_commit();
@@ -163,15 +183,14 @@ down_kernel(const X* __restrict__ x, int64_t ldx, const T* __restrict__ a, int64
           block_read(got, 16 * m + 8 * h + g, c, f);
           xv[h] = pack8<T>(f);
         }
-        if (x16 != nullptr && k < width && 16 * m + 8 * h + g < rows)
-          stg16(x16 + (t0 + 16 * m + 8 * h + g) * ldx16 + k, xv[h]);
+        if (x16 != nullptr && k < width && 16 * m + 8 * h + g < rows) stg16(x16p + (16 * m + 8 * h) * ldx16 + k, xv[h]);
       }
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         uint32_t lo[4], hi[4];
         const unsigned long long group = group0 + static_cast<unsigned long long>(2 * m * width + k / 8);
-        mask8(philox::words(key[b], group), xv[0], d.limit[b], lo);
-        mask8(philox::words(key[b], group + static_cast<unsigned long long>(width)), xv[1], d.limit[b], hi);
+        mask8(philox::words(key, ctr[b], group), xv[0], d.cut[b], d, lo);
+        mask8(philox::words(key, ctr[b], group + static_cast<unsigned long long>(width)), xv[1], d.cut[b], d, hi);
         const uint32_t f0[4] = {lo[0], hi[0], lo[1], hi[1]}, f1[4] = {lo[2], hi[2], lo[3], hi[3]};
 #pragma unroll
         for (int n = b * NTB; n < (b + 1) * NTB; ++n) {
@@ -246,12 +265,13 @@ bwd_kernel(const T* __restrict__ du, int64_t ld_du, const T* __restrict__ x16, i
   const int n = n_tok - first < chunk ? static_cast<int>(n_tok - first) : chunk;  // tokens of the chunk
   const int k = 32 * cb + 8 * c;
   const bool in = k < width;
-  philox::Key key[NB];
+  const philox::Key key = philox::make_key(rng);
+  philox::Stream ctr[NB];
   uint32_t af[NB][KR][4][2];   // A as P's operand: rows (rank) 2 c, 2 c + 1 (+ 8) of column n = g of tile j
   float acc[NB][KR][4][4];     // dA
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
-    key[b] = philox::make_key(rng, stream_id + b);
+    ctr[b] = philox::make_stream(rng, stream_id + b);
 #pragma unroll
     for (int r = 0; r < KR; ++r)
 #pragma unroll
@@ -339,6 +359,7 @@ bwd_kernel(const T* __restrict__ du, int64_t ld_du, const T* __restrict__ x16, i
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       if (d.scale[b] == 0.f) continue;  // nothing is kept
+      const uint32_t limit = d.cut[b] & 0xFFFF0000u;
       uint32_t m[2][4];
       float p[4][4] = {};
       // rows (tokens) lane & 15, rank columns 8 (lane >> 4) ..
@@ -355,14 +376,12 @@ bwd_kernel(const T* __restrict__ du, int64_t ld_du, const T* __restrict__ x16, i
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint4 w = philox::words(key[b], group + static_cast<unsigned long long>(h * width));
+        const uint4 w = philox::words(key, ctr[b], group + static_cast<unsigned long long>(h * width));
         const uint32_t ws[4] = {w.x, w.y, w.z, w.w}, xs[4] = {xv[h].x, xv[h].y, xv[h].z, xv[h].w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const bool lo = keep_lo(ws[j], d.limit[b]), hi = keep_hi(ws[j], d.limit[b]);
-          m[h][j] = mask_pair(xs[j], lo, hi);
-          if (lo) out[h][2 * j] = fmaf(d.scale[b], p[j][2 * h], out[h][2 * j]);
-          if (hi) out[h][2 * j + 1] = fmaf(d.scale[b], p[j][2 * h + 1], out[h][2 * j + 1]);
+          m[h][j] = mask_add_pair(ws[j], xs[j], limit, d.shift, d.scale[b], p[j][2 * h], p[j][2 * h + 1], out[h][2 * j],
+                                  out[h][2 * j + 1]);
         }
       }
       uint32_t bf[4][2];
@@ -463,10 +482,13 @@ Drop make_drop(double p0, double p1) {
   Drop d;
   const double p[2] = {p0, p1};
   for (int b = 0; b < 2; ++b) {
-    const uint32_t cut = philox::cut_of(p[b]);
-    d.limit[b] = cut << 16;
+    const uint32_t cut = philox::cut_of(p[b]), lane = cut < 65536u ? cut : 0u;
+    d.cut[b] = lane << 16 | lane;
     d.scale[b] = philox::scale_of(cut);
   }
+  d.ones = 0xFFFFu;
+  d.shift = 65536u;
+  d.minus = 0xFFFFFFFFu;
   return d;
 }
 
@@ -498,11 +520,11 @@ int launch_down_m(const DownArgs& p) {
   return check_launch("lora_down_dropout");
 }
 
-// Few rows: 16 a CTA, the width over 8 warps; many: 32 (lora_A is read half as often), over 4 warps.
+// Few rows: the width over 8 warps, many: over 4.
 template <typename X, typename T, int NB, int NTB>
 int launch_down_t(const DownArgs& p) {
   return p.n_tok <= 32 * static_cast<int64_t>(sm_count()) ? launch_down_m<X, T, NB, NTB, 1, 8>(p)
-                                                          : launch_down_m<X, T, NB, NTB, 2, 4>(p);
+                                                          : launch_down_m<X, T, NB, NTB, 1, 4>(p);
 }
 
 template <typename X, typename T>
