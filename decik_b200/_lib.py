@@ -111,8 +111,10 @@ SIGNATURES = {
                                               c_float, c_int, c_void_p]),
     "decik_dropout": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int, c_int64, c_double, c_void_p, c_int64,
                               c_void_p]),
+    "decik_qkv_proj_gemm": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p,
+                                    Tensor3, Tensor3, Tensor3, c_int64, c_int, c_int, c_int, c_int, c_int, c_void_p]),
     "decik_lora_down_dropout": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
-                                        c_int64, c_int64, c_int, c_int, c_int, c_double, c_double, c_void_p, c_int64,
+                                        c_int64, c_int, c_int64, c_int, c_int, c_int, c_double, c_double, c_void_p, c_int64,
                                         c_int, c_void_p]),
     "decik_lora_down_dropout_bwd_workspace": (c_int64, [c_int64, c_int, c_int, c_int]),
     "decik_lora_down_dropout_bwd": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64,

@@ -123,12 +123,16 @@ class QLoRAAttentionBlock:
         return w
 
     def forward(self, x: torch.Tensor, packing: Packing, cos: torch.Tensor, sin: torch.Tensor,
-                fused: bool = True, norm: tuple | None = None):
+                fused: bool = True, norm: tuple | None = None, dropout: tuple | None = None):
         """x fp32 [T, hidden] (the normed hidden states) -> attention output [T, n_heads*D] (dtype).
         ``fused``: one projection GEMM + the sm_100a epilogues (FusedAttentionBlock); otherwise the
         reference's chain of autograd Functions (NF4Linear x3, LoRA, FusedQKRope, VarlenSDPA).
         With ``norm`` = (weight, eps) x is the decoder layer's input and the block starts with its
-        input RMSNorm: inside the fused node's first kernel, or as RMSNormFn before the chain."""
+        input RMSNorm: inside the fused node's first kernel, or as RMSNormFn before the chain.
+        With ``dropout`` = (p_q, p_v, rng, stream) the LoRA branches of the fused node see x under
+        counter-based dropout."""
+        if dropout is not None and not fused:
+            raise RuntimeError("QLoRAAttentionBlock: counter-based dropout is the fused node's")
         dt = self.dtype
         T = x.shape[0]
         if fused:
@@ -137,7 +141,7 @@ class QLoRAAttentionBlock:
             out = FusedAttentionBlock.apply(x, a_q, b_q, a_v, b_v, self.dequant_cat(), self.bias_cat, cos, sin,
                                             packing.cu_seqlens(x.device), packing.max_len, self.n_heads,
                                             self.n_kv, self.scaling, self.head_dim ** -0.5, None, None, norm_w,
-                                            eps)
+                                            eps, None, dropout)
             return out.view(T, self.n_heads * self.head_dim)
         if norm is not None:
             from .solution.rmsnorm import RMSNormFn

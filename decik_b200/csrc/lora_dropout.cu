@@ -113,7 +113,7 @@ struct DownTile {
 template <typename X, typename T, int NB, int NTB, int MT, int WARPS>
 __global__ void __launch_bounds__(32 * WARPS, NB * NTB <= 4 ? (WARPS == 4 ? 5 : 2) : 8 / WARPS)
 down_kernel(const X* __restrict__ x, int64_t ldx, const T* __restrict__ a, int64_t lda, T* __restrict__ x16,
-            int64_t ldx16, T* __restrict__ u, int64_t ldu, int64_t n_tok, int width, int rank, Drop d,
+            int64_t ldx16, T* __restrict__ u, int64_t ldu, int u_cols, int64_t n_tok, int width, int rank, Drop d,
             const int64_t* __restrict__ rng, int64_t stream_id) {
   using Tile = DownTile<X, T, NB, NTB, MT>;
   constexpr int NT = NB * NTB, XP = Tile::kXPieces, LD = Tile::kLd;   // NT: n8 tiles of u's columns
@@ -228,6 +228,11 @@ down_kernel(const X* __restrict__ x, int64_t ldx, const T* __restrict__ a, int64
       *reinterpret_cast<uint32_t*>(u + t * ldu + b * rank + r) = scale == 0.f ? 0u : Dt<T>::pack2(s.x * scale, s.y * scale);
     }
   }
+  // the columns behind the branches': a 1 (it multiplies the bias in the projection's extra K block), zeros
+  const int n_u = NB * rank, more = (u_cols - n_u) / 2;
+  for (int i = threadIdx.x; i < rows * more; i += 32 * WARPS)
+    *reinterpret_cast<uint32_t*>(u + (t0 + i / more) * ldu + n_u + 2 * (i % more)) =
+        i % more == 0 ? Dt<T>::pack2(1.f, 0.f) : 0u;
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -500,7 +505,9 @@ struct DownArgs {
   void* x16;
   int64_t ldx16;
   void* u;
-  int64_t ldu, n_tok;
+  int64_t ldu;
+  int u_cols;
+  int64_t n_tok;
   int width, rank;
   Drop d;
   const int64_t* rng;
@@ -516,7 +523,7 @@ int launch_down_m(const DownArgs& p) {
   if (int rc = ensure_dyn_smem(kernel, smem, done, "lora_down_dropout")) return rc;
   kernel<<<static_cast<unsigned>((p.n_tok + 16 * MT - 1) / (16 * MT)), 32 * WARPS, smem, p.s>>>(
       static_cast<const X*>(p.x), p.ldx, static_cast<const T*>(p.a), p.lda, static_cast<T*>(p.x16), p.ldx16,
-      static_cast<T*>(p.u), p.ldu, p.n_tok, p.width, p.rank, p.d, p.rng, p.stream_id);
+      static_cast<T*>(p.u), p.ldu, p.u_cols, p.n_tok, p.width, p.rank, p.d, p.rng, p.stream_id);
   return check_launch("lora_down_dropout");
 }
 
@@ -539,23 +546,25 @@ int launch_down(const DownArgs& p, int branches) {
 }  // namespace decik
 
 extern "C" int decik_lora_down_dropout(const void* x, int x_dtype, int64_t ldx, const void* a, int64_t lda, void* x16,
-                                       int64_t ldx16, void* u, int64_t ldu, int64_t n_tok, int width, int rank,
-                                       int n_branch, double p0, double p1, const int64_t* rng, int64_t stream_id,
+                                       int64_t ldx16, void* u, int64_t ldu, int u_cols, int64_t n_tok, int width,
+                                       int rank, int n_branch, double p0, double p1, const int64_t* rng, int64_t stream_id,
                                        int dtype, void* stream) {
   using namespace decik;
   using namespace decik::loradrop;
   if (int rc = check_sizes("lora_down_dropout", n_tok, width, rank, n_branch, p0, p1, dtype)) return rc;
   if (x_dtype != DECIK_F32 && x_dtype != dtype)
     return set_error(DECIK_ERR_INVALID, "lora_down_dropout: x of dtype %d (F32 or the compute dtype %d)", x_dtype, dtype);
+  if (u_cols < rank * n_branch || u_cols % 8 != 0)
+    return set_error(DECIK_ERR_INVALID, "lora_down_dropout: u_cols %d (a multiple of 8 from %d on)", u_cols, rank * n_branch);
   if (n_tok == 0) return DECIK_OK;
   if (!x || !a || !u || !rng) return set_error(DECIK_ERR_INVALID, "lora_down_dropout: null pointer");
-  if (ldx < width || lda < width || (x16 && ldx16 < width) || ldu < rank * n_branch)
+  if (ldx < width || lda < width || (x16 && ldx16 < width) || ldu < u_cols)
     return set_error(DECIK_ERR_INVALID, "lora_down_dropout: row strides shorter than the rows");
   const int xe = x_dtype == DECIK_F32 ? 4 : 8;
   if (ldx % xe || lda % 8 || (x16 && ldx16 % 8) || ldu % 8 || !aligned16(x) || !aligned16(a) ||
       (x16 && !aligned16(x16)) || !aligned16(u))
     return set_error(DECIK_ERR_INVALID, "lora_down_dropout: rows and pointers need 16-byte alignment");
-  const DownArgs p{x, ldx, a, lda, x16, ldx16, u, ldu, n_tok, width, rank, make_drop(p0, p1), rng, stream_id,
+  const DownArgs p{x, ldx, a, lda, x16, ldx16, u, ldu, u_cols, n_tok, width, rank, make_drop(p0, p1), rng, stream_id,
                    as_stream(stream)};
   return DECIK_DISPATCH_16(dtype, [&] {
     return x_dtype == DECIK_F32 ? launch_down<float, T>(p, n_branch) : launch_down<T, T>(p, n_branch);

@@ -742,8 +742,8 @@ __global__ void __launch_bounds__(kCastThreads) x_cast_lora_down_kernel(const fl
 // ------------------------------------------------------------------------------------------------
 // dA = du^T x16, dB = scaling g^T u: reductions over the tokens on mma.sync
 // ------------------------------------------------------------------------------------------------
-// Output row block v (blockIdx.y): v < hidden / 128 -> dA^T rows (hidden columns 128 v ..): P = x16,
-// Q = du (32 columns); else dB rows of lora_B head v - hidden / 128 (q heads, then v heads): P = the
+// Output row block v (blockIdx.y): v < n_da (hidden / 128, or 0 without dA) -> dA^T rows (hidden columns
+// 128 v ..): P = x16, Q = du (32 columns); else dB rows of lora_B head v - n_da (q heads, then v heads): P = the
 // head's g columns of dy, Q = u_q or u_v (16 columns). out[m][n] += sum_t P[t][m] Q[t][n] over the
 // block's token chunk (blockIdx.x), added into fp32 outputs zeroed by the caller.
 constexpr int kGradTok = 512, kGradStep = 64, kGradThreads = 256, kPLd = 128 + 8, kQLd = 32 + 8;
@@ -753,11 +753,11 @@ __global__ void __launch_bounds__(kGradThreads) lora_grad_kernel(const T* __rest
                                                                  const T* __restrict__ x16, int64_t ldx,
                                                                  const T* __restrict__ u, int64_t ldu, float* __restrict__ da,
                                                                  float* __restrict__ db, float scaling,
-                                                                 int64_t n_tok, int hidden, int hq, int hk) {
+                                                                 int64_t n_tok, int hidden, int hq, int hk, int n_da) {
   __shared__ __align__(16) T ps[2][kGradStep * kPLd];
   __shared__ __align__(16) T qs[2][kGradStep * kQLd];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int vb = blockIdx.y, n_da = hidden / kD;
+  const int vb = blockIdx.y;
   const bool is_a = vb < n_da;
   const int head = vb - n_da;  // dB: lora_B head slot (q heads, then v heads)
   const int nq = is_a ? 2 * kR : kR;  // Q columns
@@ -963,7 +963,8 @@ int launch_cast(const float* x, int64_t ldx, const T* a16, int64_t lda, T* x16, 
   return check_launch(norm_w == nullptr ? "x_cast_lora_down" : "rmsnorm_cast_lora_down");
 }
 
-int qkv_proj_fwd_impl(const float* x, int64_t ldx, const void* norm_w, int norm_dtype, float eps, float* rstd,
+// with cast false x16 and u are the caller's (decik_qkv_proj_gemm), and only the GEMM runs
+int qkv_proj_fwd_impl(bool cast, const float* x, int64_t ldx, const void* norm_w, int norm_dtype, float eps, float* rstd,
                       const void* w_cat, int64_t ldw, const void* ext_b, int lora, const float* cosp,
                       const float* sinp, decik_tensor3_mut q, decik_tensor3_mut k, decik_tensor3_mut v, void* x16,
                       int64_t ldx16, void* u, int64_t n_tok, int hidden, int n_heads, int n_kv, int head_dim,
@@ -973,9 +974,9 @@ int qkv_proj_fwd_impl(const float* x, int64_t ldx, const void* norm_w, int norm_
       hidden <= 0 || hidden % 128 != 0 || (n_heads + 2 * n_kv) % 2 != 0)
     return set_error(DECIK_ERR_INVALID, "qkv_proj_fwd: T=%lld hidden %d heads %d/%d head_dim %d (needs head_dim 128, "
                      "hidden %% 128 == 0, an even head count)", (long long)n_tok, hidden, n_heads, n_kv, head_dim);
-  if (!x || !w_cat || !ext_b || !cosp || !sinp || !q.ptr || !k.ptr || !v.ptr || !x16 || !u)
+  if ((cast && !x) || !w_cat || !ext_b || !cosp || !sinp || !q.ptr || !k.ptr || !v.ptr || !x16 || !u)
     return set_error(DECIK_ERR_INVALID, "qkv_proj_fwd: NULL pointer");
-  if (ldx < hidden || ldw < hidden || ldx16 < hidden)
+  if ((cast && ldx < hidden) || ldw < hidden || ldx16 < hidden)
     return set_error(DECIK_ERR_INVALID, "qkv_proj_fwd: row strides shorter than hidden");
   if (ldx % 4 || ldw % 8 || ldx16 % 8 || !aligned16(x) || !aligned16(w_cat) || !aligned16(x16) || !aligned16(u) ||
       !aligned16(ext_b) || !aligned16(cosp) || !aligned16(sinp))
@@ -1020,6 +1021,7 @@ int qkv_proj_fwd_impl(const float* x, int64_t ldx, const void* norm_w, int norm_
   const int64_t a_off = static_cast<int64_t>(n_proj) * ldw;
   if (dtype == DECIK_BF16) {
     using T = __nv_bfloat16;
+    if (!cast) return launch_gemm<T, EPI_QKV, true>(p, s, "qkv_proj_gemm");
     if (int rc = launch_cast<T>(x, ldx, lora ? static_cast<const T*>(w_cat) + a_off : nullptr, ldw,
                                 static_cast<T*>(x16), ldx16, static_cast<T*>(u), n_tok, hidden, norm_w, norm_dtype,
                                 eps, rstd, s))
@@ -1027,6 +1029,7 @@ int qkv_proj_fwd_impl(const float* x, int64_t ldx, const void* norm_w, int norm_
     return launch_gemm<T, EPI_QKV, true>(p, s, "qkv_proj_gemm");
   }
   using T = __half;
+  if (!cast) return launch_gemm<T, EPI_QKV, true>(p, s, "qkv_proj_gemm");
   if (int rc = launch_cast<T>(x, ldx, lora ? static_cast<const T*>(w_cat) + a_off : nullptr, ldw,
                               static_cast<T*>(x16), ldx16, static_cast<T*>(u), n_tok, hidden, norm_w, norm_dtype, eps,
                               rstd, s))
@@ -1043,7 +1046,7 @@ extern "C" int decik_qkv_proj_fwd(const float* x, int64_t ldx, const void* w_cat
                                   decik_tensor3_mut k, decik_tensor3_mut v, void* x16, int64_t ldx16, void* u,
                                   int64_t n_tok, int hidden, int n_heads, int n_kv, int head_dim, int dtype,
                                   void* stream) {
-  return decik::proj::qkv_proj_fwd_impl(x, ldx, nullptr, 0, 0.f, nullptr, w_cat, ldw, ext_b, lora, cosp, sinp, q, k,
+  return decik::proj::qkv_proj_fwd_impl(true, x, ldx, nullptr, 0, 0.f, nullptr, w_cat, ldw, ext_b, lora, cosp, sinp, q, k,
                                         v, x16, ldx16, u, n_tok, hidden, n_heads, n_kv, head_dim, dtype, stream);
 }
 
@@ -1054,8 +1057,17 @@ extern "C" int decik_qkv_proj_norm_fwd(const float* h, int64_t ldh, const void* 
                                        int hidden, int n_heads, int n_kv, int head_dim, int dtype, void* stream) {
   if (n_tok != 0 && (norm_w == nullptr || rstd == nullptr))
     return decik::set_error(DECIK_ERR_INVALID, "qkv_proj_norm_fwd: NULL norm weight or rstd");
-  return decik::proj::qkv_proj_fwd_impl(h, ldh, norm_w, norm_dtype, eps, rstd, w_cat, ldw, ext_b, lora, cosp, sinp, q,
+  return decik::proj::qkv_proj_fwd_impl(true, h, ldh, norm_w, norm_dtype, eps, rstd, w_cat, ldw, ext_b, lora, cosp, sinp, q,
                                         k, v, x16, ldx16, u, n_tok, hidden, n_heads, n_kv, head_dim, dtype, stream);
+}
+
+extern "C" int decik_qkv_proj_gemm(const void* x16, int64_t ldx16, const void* u, const void* w_cat, int64_t ldw,
+                                   const void* ext_b, const float* cosp, const float* sinp, decik_tensor3_mut q,
+                                   decik_tensor3_mut k, decik_tensor3_mut v, int64_t n_tok, int hidden, int n_heads,
+                                   int n_kv, int head_dim, int dtype, void* stream) {
+  return decik::proj::qkv_proj_fwd_impl(false, nullptr, 0, nullptr, 0, 0.f, nullptr, w_cat, ldw, ext_b, 0, cosp, sinp, q,
+                                        k, v, const_cast<void*>(x16), ldx16, const_cast<void*>(u), n_tok, hidden,
+                                        n_heads, n_kv, head_dim, dtype, stream);
 }
 
 extern "C" int decik_proj_dx(const void* dy, int64_t ld_dy, int k_cols, const void* w_t, int64_t ldw, float* dx,
@@ -1097,27 +1109,28 @@ extern "C" int decik_lora_grads(const void* dy, int64_t ld_dy, const void* x16, 
   using namespace decik::proj;
   if (n_tok < 0 || hidden <= 0 || hidden % kD != 0 || n_heads <= 0 || n_kv <= 0)
     return set_error(DECIK_ERR_INVALID, "lora_grads: T=%lld hidden %d heads %d/%d", (long long)n_tok, hidden, n_heads, n_kv);
-  if (!dy || !x16 || !u || !da || !db) return set_error(DECIK_ERR_INVALID, "lora_grads: NULL pointer");
+  if (!dy || !x16 || !u || !db) return set_error(DECIK_ERR_INVALID, "lora_grads: NULL pointer");
   if (ld_dy < static_cast<int64_t>(n_heads + 2 * n_kv) * kD + 2 * kR || ldx < hidden)
     return set_error(DECIK_ERR_INVALID, "lora_grads: dy rows need (heads + 2 kv heads) x 128 + 32 columns, x16 rows hidden");
   if (ld_dy % 8 || ldx % 8 || ldu % 8 || ldu < 2 * kR || !aligned16(dy) || !aligned16(x16) || !aligned16(u))
     return set_error(DECIK_ERR_INVALID, "lora_grads: rows and pointers need 16-byte alignment (u rows >= 32)");
   cudaStream_t s = as_stream(stream);
-  cudaError_t e = cudaMemsetAsync(da, 0, sizeof(float) * 2 * kR * hidden, s);
+  cudaError_t e = da == nullptr ? cudaSuccess : cudaMemsetAsync(da, 0, sizeof(float) * 2 * kR * hidden, s);
   if (e == cudaSuccess) e = cudaMemsetAsync(db, 0, sizeof(float) * (n_heads + n_kv) * kD * kR, s);
   if (e != cudaSuccess) return set_error(DECIK_ERR_CUDA, "lora_grads: memset: %s", cudaGetErrorString(e));
   if (n_tok == 0) return DECIK_OK;
-  const dim3 grid(static_cast<unsigned>((n_tok + kGradTok - 1) / kGradTok), hidden / kD + n_heads + n_kv);
+  const int n_da = da == nullptr ? 0 : hidden / kD;
+  const dim3 grid(static_cast<unsigned>((n_tok + kGradTok - 1) / kGradTok), n_da + n_heads + n_kv);
   if (dtype == DECIK_BF16) {
     using T = __nv_bfloat16;
     lora_grad_kernel<T><<<grid, kGradThreads, 0, s>>>(static_cast<const T*>(dy), ld_dy, static_cast<const T*>(x16),
                                                       ldx, static_cast<const T*>(u), ldu, da, db, scaling, n_tok, hidden,
-                                                      n_heads, n_kv);
+                                                      n_heads, n_kv, n_da);
   } else if (dtype == DECIK_F16) {
     using T = __half;
     lora_grad_kernel<T><<<grid, kGradThreads, 0, s>>>(static_cast<const T*>(dy), ld_dy, static_cast<const T*>(x16),
                                                       ldx, static_cast<const T*>(u), ldu, da, db, scaling, n_tok, hidden,
-                                                      n_heads, n_kv);
+                                                      n_heads, n_kv, n_da);
   } else {
     return set_error(DECIK_ERR_INVALID, "lora_grads: dtype %d", dtype);
   }

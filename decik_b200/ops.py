@@ -473,12 +473,14 @@ def _branches(what: str, a: torch.Tensor, p, width: int):
     return a.shape[0] // len(ps), len(ps), ps if len(ps) == 2 else (ps[0], 0.0)
 
 
-def lora_down_dropout(x: torch.Tensor, a: torch.Tensor, p, rng: torch.Tensor, stream: int = 0):
+def lora_down_dropout(x: torch.Tensor, a: torch.Tensor, p, rng: torch.Tensor, stream: int = 0,
+                      u_cols: int | None = None):
     """The LoRA down projections of x [T, W] (fp32, or a's dtype) under counter-based dropout
     (decik_lora_down_dropout): a [branches * rank, W] of fp16 / bf16 holds the branches' lora_A, ``p``
     the probability of each (a number or a tuple); branch b has the mask of (rng, stream + b) over x.
     Returns x16 = x in a's dtype (x itself where it has it) and u [T, branches * rank] =
-    scale_b (keep_b x16) A_b^T."""
+    scale_b (keep_b x16) A_b^T; with ``u_cols`` (64 for qkv_proj_gemm) u has that many columns, a 1 and
+    zeros behind the branches'."""
     what = "lora_down_dropout"
     dev = _device(what, x, a, rng)
     _check_rng(what, rng)
@@ -489,9 +491,11 @@ def lora_down_dropout(x: torch.Tensor, a: torch.Tensor, p, rng: torch.Tensor, st
     T, W = x.shape
     rank, nb, ps = _branches(what, a, p, W)
     x16 = x if x.dtype == a.dtype else a.new_empty((T, W))
-    u = a.new_empty((T, nb * rank))
+    u_cols = nb * rank if u_cols is None else u_cols
+    u = a.new_empty((T, u_cols))
     _launch(what, 1, dev, _lib.lib().decik_lora_down_dropout, x.data_ptr(), _dt(x), _ld(x), a.data_ptr(), _ld(a),
-            None if x16 is x else x16.data_ptr(), W, u.data_ptr(), nb * rank, T, W, rank, nb, *ps, rng.data_ptr(),
+            None if x16 is x else x16.data_ptr(), W, u.data_ptr(), u_cols, u_cols, T, W, rank, nb, *ps,
+            rng.data_ptr(),
             stream, _dt(a))
     return x16, u
 
@@ -823,6 +827,27 @@ def qkv_proj_fwd(x: torch.Tensor, w_cat: torch.Tensor, ext_b: torch.Tensor, lora
     return x16, u, q, k, v, rstd
 
 
+def qkv_proj_gemm(x16: torch.Tensor, u: torch.Tensor, w_cat: torch.Tensor, ext_b: torch.Tensor, cos: torch.Tensor,
+                  sin: torch.Tensor, n_heads: int, n_kv: int):
+    """q [Hq, T, D], k [Hk, T, D], v [T, Hk, D] of qkv_proj_fwd from a caller's x16 [T, H] and u [T, 64]
+    (u_q | u_v | 1 | zeros, lora_down_dropout's with u_cols 64): its GEMM alone (decik_qkv_proj_gemm)."""
+    _cuda(x16, u, w_cat, ext_b, cos, sin)
+    T, H = x16.shape
+    D = cos.shape[-1]
+    if u.shape != (T, 4 * LORA_RANK) or not u.is_contiguous() or x16.stride(1) != 1 or w_cat.stride(1) != 1:
+        raise RuntimeError("decik_b200 qkv_proj_gemm: u contiguous [T, 64], x16 and w_cat with contiguous rows")
+    q = torch.empty((n_heads, T, D), dtype=x16.dtype, device=x16.device)
+    k = torch.empty((n_kv, T, D), dtype=x16.dtype, device=x16.device)
+    v = torch.empty((T, n_kv, D), dtype=x16.dtype, device=x16.device)
+    with _timed("qkv_proj_gemm", 1):
+        rc = _lib.lib().decik_qkv_proj_gemm(
+            _p(x16), x16.stride(0), _p(u), _p(w_cat), w_cat.stride(0), _p(ext_b), _p(cos.contiguous()),
+            _p(sin.contiguous()), _t3any(q.transpose(0, 1)), _t3any(k.transpose(0, 1)), _t3any(v), T, H, n_heads, n_kv, D,
+            _dt(x16), _stream(x16))
+    _lib.check(rc, "qkv_proj_gemm")
+    return q, k, v
+
+
 def transpose16(src: torch.Tensor) -> torch.Tensor:
     """src [R, C] (16-bit, contiguous rows) -> a new [C, R] tensor (decik_transpose16)."""
     _cuda(src)
@@ -900,13 +925,15 @@ def mlp_down_grad(grad16: torch.Tensor, w_down: torch.Tensor, gu: torch.Tensor) 
     return dgu
 
 
-def lora_grads(dy: torch.Tensor, x16: torch.Tensor, u: torch.Tensor, scaling: float, n_heads: int, n_kv: int):
+def lora_grads(dy: torch.Tensor, x16: torch.Tensor, u: torch.Tensor, scaling: float, n_heads: int, n_kv: int,
+               want_da: bool = True):
     """(dA [32, H], dB [(Hq+Hk)*D, 16]) fp32 of the fused block (decik_lora_grads): dA = du^T x16 with
-    du = dy's last 32 columns; dB = scaling g^T u over dy's q columns (u_q) and v columns (u_v)."""
+    du = dy's last 32 columns (None without ``want_da``); dB = scaling g^T u over dy's q columns (u_q) and
+    v columns (u_v)."""
     _cuda(dy, x16, u)
     T, H = x16.shape
     D = 128
-    da = torch.empty((2 * LORA_RANK, H), dtype=torch.float32, device=dy.device)
+    da = torch.empty((2 * LORA_RANK, H), dtype=torch.float32, device=dy.device) if want_da else None
     db = torch.empty(((n_heads + n_kv) * D, LORA_RANK), dtype=torch.float32, device=dy.device)
     with _timed("lora_grads", 1):
         if u.stride(1) != 1:

@@ -15,6 +15,11 @@ class _State:
         # whether the packed attention runs on the varlen kernels (varlen.patch's switch); the fused
         # attention block calls them directly, so it follows the same switch
         self.varlen_attention = False
+        # counter-based dropout (dropout.py): the switch (a seed or True), the generator by device, and the
+        # streams of the packed forward that runs (dropout.StepStreams), None while the masks are torch's
+        self.counter_dropout = None
+        self.counter_rngs = {}
+        self.dropout = None
 
 
 STATE = _State()

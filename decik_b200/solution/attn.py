@@ -100,7 +100,7 @@ class AxesRope(torch.autograd.Function):
 
 class FusedAttentionBlock(torch.autograd.Function):
     """x -> packed causal GQA attention output [T, Hq, D] in one autograd node, for q/v LoRA
-    without dropout. The arithmetic of the reference's chain (solution/attn.py:395-416: three
+    without dropout or with counter-based dropout. The arithmetic of the reference's chain (solution/attn.py:395-416: three
     NF4Linear, LoRAPairFromNorm, FusedQKRope, VarlenSDPA), regrouped so each pass over the tokens
     does as much as it can:
 
@@ -127,11 +127,18 @@ class FusedAttentionBlock(torch.autograd.Function):
     norm's backward (decik_rmsnorm_bwd, from the kept rstd) to dX and returns the gradient for h.
     The LoRA gradients use the kept x16, so there is no norm recompute (solution/attn.py:238).
     With ``residual_link`` (rmsnorm.ResidualGradLink, armed here) h's gradient from the residual
-    stream, left there by the layer's AddRMSNormFn, is added in the same pass."""
+    stream, left there by the layer's AddRMSNormFn, is added in the same pass.
+
+    With ``dropout`` = (p_q, p_v, rng, stream) the LoRA branches see x16 under counter-based dropout
+    (streams ``stream`` and ``stream + 1`` of the generator state ``rng``): u comes from
+    decik_lora_down_dropout (after a norm pass of its own), the GEMM is decik_qkv_proj_gemm, and in
+    backward the branches' input gradient and dA come from decik_lora_down_dropout_bwd, which adds to
+    the dX of the three projections in place and computes the masks again."""
 
     @staticmethod
     def forward(ctx, x, a_q, b_q, a_v, b_v, w_cat, bias_cat, cos, sin, cu_seqlens, max_len, n_heads,
-                n_kv, scaling, scale, w_o=None, b_o=None, norm_w=None, norm_eps=0.0, residual_link=None):
+                n_kv, scaling, scale, w_o=None, b_o=None, norm_w=None, norm_eps=0.0, residual_link=None,
+                dropout=None):
         dt = w_cat.dtype
         ctx.link = residual_link if norm_w is not None else None
         if ctx.link is not None:
@@ -142,7 +149,15 @@ class FusedAttentionBlock(torch.autograd.Function):
         frag = ops.lora_pack(a_q, a_v, b_q, b_v, dt, a_out=w_cat[n_proj:])
         ext_b = ops.lora_b_ext(b_q, b_v, scaling, bias_cat, dt, n_heads, n_kv)  # scaled lora_B + bias
         x32 = x if (x.dtype == torch.float32 and x.stride(-1) == 1) else x.float().contiguous()
-        if norm_w is None:
+        if dropout is not None:
+            y32, h, rstd = x32, None, None
+            if norm_w is not None:
+                h = x32
+                y32, rstd = ops.rmsnorm_fwd(h, norm_w, norm_eps)
+            p_q, p_v, rng, stream = dropout
+            x16, u = ops.lora_down_dropout(y32, w_cat[n_proj:], (p_q, p_v), rng, stream, u_cols=64)
+            q, k, v = ops.qkv_proj_gemm(x16, u, w_cat, ext_b, cos, sin, n_heads, n_kv)
+        elif norm_w is None:
             x16, u, q, k, v = ops.qkv_proj_fwd(x32, w_cat, ext_b, True, cos, sin, n_heads, n_kv)
             h = rstd = None
         else:
@@ -150,15 +165,17 @@ class FusedAttentionBlock(torch.autograd.Function):
                                                      norm=(norm_w, norm_eps))
             h = x32
         out, lse = ops.varlen_attn_fwd(q.transpose(0, 1), k.transpose(0, 1), v, cu_seqlens, max_len, scale)
-        ctx.save_for_backward(x16, w_cat, u, frag, cos, sin, q, k, v, out, lse, cu_seqlens, w_o, h, norm_w, rstd)
+        ctx.save_for_backward(x16, w_cat, u, frag, cos, sin, q, k, v, out, lse, cu_seqlens, w_o, h, norm_w, rstd,
+                              None if dropout is None else dropout[2])
         ctx.meta = (int(max_len), n_heads, n_kv, float(scaling), float(scale), r)
+        ctx.dropout = None if dropout is None else (dropout[0], dropout[1], dropout[3])
         if w_o is not None:
             return F.linear(out.view(out.shape[0], -1), w_o, b_o)
         return out
 
     @staticmethod
     def backward(ctx, grad_out):
-        x16, w_cat, u, frag, cos, sin, q, k, v, out, lse, cu, w_o, h, norm_w, rstd = ctx.saved_tensors
+        x16, w_cat, u, frag, cos, sin, q, k, v, out, lse, cu, w_o, h, norm_w, rstd, rng = ctx.saved_tensors
         max_len, n_heads, n_kv, scaling, scale, r = ctx.meta
         if w_o is not None:  # through o_proj first: the attention output's gradient
             grad_out = torch.mm(grad_out.reshape(-1, grad_out.shape[-1]).to(w_o.dtype), w_o).view(out.shape)
@@ -172,11 +189,18 @@ class FusedAttentionBlock(torch.autograd.Function):
         # from their place in dy
         ops.attn_qkv_bwd(g, q.transpose(0, 1), k.transpose(0, 1), v, out, lse, cu, max_len, scale, cos, sin,
                          frag, scaling, dy)
-        dx = ops.proj_dx(dy, ops.transpose16(w_cat))
-        da, db = ops.lora_grads(dy, x16, u, scaling, n_heads, n_kv)
+        if ctx.dropout is None:
+            dx = ops.proj_dx(dy, ops.transpose16(w_cat))
+            da, db = ops.lora_grads(dy, x16, u, scaling, n_heads, n_kv)
+        else:  # the LoRA branches' part goes through their masks
+            p_q, p_v, stream = ctx.dropout
+            dx = ops.proj_dx(dy, ops.transpose16(w_cat[:n_proj]))
+            dx, da = ops.lora_down_dropout_bwd(dy[:, n_proj:], x16, w_cat[n_proj:], (p_q, p_v), rng, stream, addend=dx,
+                                               out=dx)
+            _, db = ops.lora_grads(dy, x16, u, scaling, n_heads, n_kv, want_da=False)
         if norm_w is not None:  # through the input norm: the gradient for the layer input h
             dx = ops.rmsnorm_bwd(dx, h, norm_w, rstd, addend=None if ctx.link is None else ctx.link.take())
-        return (dx, da[:r], db[:n_q], da[r:], db[n_q:]) + (None,) * 15
+        return (dx, da[:r], db[:n_q], da[r:], db[n_q:]) + (None,) * 16
 
 
 def pack_keep(keep_q, keep_v):
@@ -342,7 +366,8 @@ def _nf4_parts(module, n_in, dtype):
 def _fused_block(self, x, q_name, v_name, cos, sin, packing, dtype, n_heads, n_kv, head_dim, o_nf4=False,
                  input_norm=None, residual_link=None):
     """(output, o_proj applied) through FusedAttentionBlock, or None when this layer does not
-    qualify: both LoRA branches without dropout, rank 16 and one scaling; q, k, v NF4 linears of the
+    qualify: both LoRA branches without dropout (any with the counter-based generator on), rank 16 and
+    one scaling; q, k, v NF4 linears of the
     compute dtype; the varlen attention switched on; head_dim 128. With ``o_nf4`` (o_proj is a plain
     NF4 Linear4bit of the compute dtype) o_proj joins the node: the output is then [1, T, H].
     With ``input_norm`` (the decoder layer's input RMSNorm module, eligible for the fused kernel)
@@ -351,7 +376,7 @@ def _fused_block(self, x, q_name, v_name, cos, sin, packing, dtype, n_heads, n_k
 
     pq, pv = _lora_parts(self.q_proj, q_name), _lora_parts(self.v_proj, v_name)
     if not (STATE.varlen_attention and head_dim == 128 and pq is not None and pv is not None
-            and pq[3] == 0.0 and pv[3] == 0.0 and pq[2] == pv[2]
+            and (pq[3] == pv[3] == 0.0 or STATE.dropout is not None) and pq[2] == pv[2]
             and pq[0].shape[0] == 16 and pv[0].shape[0] == 16
             and (not self.training or getattr(self, "attention_dropout", 0.0) == 0.0)):
         return None
@@ -383,14 +408,16 @@ def _fused_block(self, x, q_name, v_name, cos, sin, packing, dtype, n_heads, n_k
                                     self.scaling, w_o, b_o,
                                     None if input_norm is None else input_norm.weight,
                                     0.0 if input_norm is None else float(input_norm.variance_epsilon),
-                                    residual_link)
+                                    residual_link,
+                                    None if pq[3] == pv[3] == 0.0 else (pq[3], pv[3], *STATE.dropout.streams(2)))
     return out.reshape(1, n_tok, -1), w_o is not None
 
 
 def patch(recompute_lora=True, linear4bit_cls=None, lora_classes=None, fused_block=True):
     """Patch Qwen2Attention.forward (solution/attn.py:349-421). ``linear4bit_cls`` and
     ``lora_classes`` default to bitsandbytes' Linear4bit and peft's LoRA layers. With
-    ``fused_block`` a qualifying layer (LoRA without dropout) runs as one FusedAttentionBlock;
+    ``fused_block`` a qualifying layer (LoRA without dropout, or with the counter-based generator on)
+    runs as one FusedAttentionBlock;
     the others keep the reference's chain of autograd Functions."""
     from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
     from transformers.models.qwen2 import modeling_qwen2

@@ -12,6 +12,9 @@ from __future__ import annotations
 import torch
 
 from .. import ops
+from ._state import STATE
+
+STREAMS = 1 << 20  # of one packed forward: its dropouts take them one after the other
 
 
 class CounterRNG:
@@ -29,6 +32,42 @@ class CounterRNG:
         now = self.state.clone()
         self.state[1] += n
         return now
+
+
+class StepStreams:
+    """The streams of one packed forward: the generator's state at its start, and the next stream."""
+
+    def __init__(self, rng: torch.Tensor):
+        self.rng, self.next = rng, 0
+
+    def streams(self, n: int):
+        """(rng, first stream) of the next n streams."""
+        first, self.next = self.next, self.next + n
+        if self.next > STREAMS:
+            raise RuntimeError(f"decik_b200 dropout: more than {STREAMS} dropouts in one forward")
+        return self.rng, first
+
+
+def step_streams(device):
+    """The StepStreams of a packed forward on ``device``, or None while counter-based dropout is off."""
+    if STATE.counter_dropout is None:
+        return None
+    rng = STATE.counter_rngs.get(device)
+    if rng is None:
+        seed = None if STATE.counter_dropout is True else STATE.counter_dropout
+        rng = STATE.counter_rngs[device] = CounterRNG(seed, device)
+    return StepStreams(rng.take(STREAMS))
+
+
+def use_counter_dropout(on=True) -> None:
+    """Switch the packed path's dropout to the counter-based generator: ``True`` (seeded by
+    torch.initial_seed()) or a seed; False switches back to torch's draws. Dropout on the packed
+    decoder (nn.Dropout, and the LoRA branches of the fused attention block, which then takes layers with
+    LoRA dropout too) draws at the real tokens only, stores no mask, and does not touch torch's
+    generators. Each packed forward takes new streams. Ranks of a data-parallel job give different
+    seeds."""
+    STATE.counter_dropout = None if on is False or on is None else on
+    STATE.counter_rngs = {}
 
 
 class CounterDropout(torch.autograd.Function):

@@ -13,7 +13,8 @@ the row lengths), one copy into pinned memory, where the reference's ``plan()``
 runs the sm_100a varlen kernels: GQA without expanding K/V, dK/dV summed over each kv head's query
 heads inside the kernel, and the forward's logsumexp kept for backward (no forward recompute).
 
-LoRA dropout on the packed path draws its random numbers exactly as the unpacked model would:
+LoRA dropout on the packed path draws its random numbers, unless counter-based dropout is switched on
+(dropout.py), exactly as the unpacked model would:
 ``torch.native_dropout`` on a [B, S, width] tensor, the op and shape of the base model's draw, of
 which only the real tokens' rows are used. So the RNG stream, and the training run, stay the same
 as the reference's.
@@ -27,6 +28,7 @@ import torch
 
 from .. import ops
 from ._state import STATE, on_gpu
+from .dropout import CounterDropout, step_streams
 
 
 class PackedBatch:
@@ -221,11 +223,13 @@ class _PackedStep:
 
     def __enter__(self):
         STATE.packing, STATE.packing_active = self.packing, True
+        STATE.dropout = step_streams(self.packing.index.device)
         return self.packing
 
     def __exit__(self, *exc):
         STATE.packing_active = False
         STATE.norm_link = None
+        STATE.dropout = None
         return False
 
 
@@ -333,6 +337,8 @@ def _decoder_layer(original, fuse_residual, fuse_input_norm=True):
 def _dropout(original):
     def forward(self, input):
         if (self.training and 0.0 < self.p < 1.0 and not self.inplace and _on_packed_path(input)):
+            if STATE.dropout is not None:
+                return CounterDropout.apply(input, self.p, *STATE.dropout.streams(1))
             values, keep = STATE.packing.dropout_draw(self.p, input.shape[-1], input.dtype, input.device)
             return PackedDropout.apply(input, values[None], keep[None], self.p)
         return original(self, input)

@@ -406,6 +406,14 @@ DECIK_API int decik_qkv_proj_norm_fwd(const float* h, int64_t ldh, const void* n
                                       decik_tensor3_mut v, void* x16, int64_t ldx16, void* u, int64_t n_tok,
                                       int hidden, int n_heads, int n_kv, int head_dim, int dtype, void* stream);
 
+/* The GEMM of decik_qkv_proj_fwd alone, for a caller's x16 [T, hidden] (ldx16) and u [T, 64] contiguous:
+ * u_q | u_v | 1 | 0 ..., made under dropout by decik_lora_down_dropout. The other arguments are
+ * decik_qkv_proj_fwd's. */
+DECIK_API int decik_qkv_proj_gemm(const void* x16, int64_t ldx16, const void* u, const void* w_cat, int64_t ldw,
+                                  const void* ext_b, const float* cosp, const float* sinp, decik_tensor3_mut q,
+                                  decik_tensor3_mut k, decik_tensor3_mut v, int64_t n_tok, int hidden, int n_heads,
+                                  int n_kv, int head_dim, int dtype, void* stream);
+
 /* dx = dy[:, 0:k_cols] . w_t[:, 0:k_cols]^T in fp32 [T, hidden] (ld_dx), w_t dt [hidden, >= k_cols]
  * (ldw) the TRANSPOSED weight (decik_transpose16 of W_cat [k_cols, hidden]): the three NF4Linear
  * input gradients (solution/nf4.py:99-104: g16 @ W16) and both LoRA input gradients
@@ -419,7 +427,8 @@ DECIK_API int decik_transpose16(const void* src, int64_t lds, void* dst, int64_t
                                 void* stream);
 
 /* The LoRA parameter gradients of the fused block (solution/attn.py:255-262):
- *   da [32, hidden] fp32 = du^T x16 (du = dy[:, n_proj : n_proj + 32]; rows 0-15 dA_q, 16-31 dA_v)
+ *   da [32, hidden] fp32 = du^T x16 (du = dy[:, n_proj : n_proj + 32]; rows 0-15 dA_q, 16-31 dA_v),
+ *      or NULL: db alone
  *   db [(n_heads + n_kv) 128, 16] fp32 = scaling . g^T u (g = dy's q columns with u_q, then its v
  *      columns with u_v)
  * dy dt [T, >= n_proj + 32] (ld_dy), x16 dt [T, hidden], u dt [T, >= 32] (ldu). Zeroes da and db,
@@ -476,7 +485,8 @@ DECIK_API int decik_dropout(const void* x, int x_dtype, const void* residual, vo
  * mask, that of stream_id + b over the [n_tok, width] input, and its own p:
  *   x16 = dt(x),  u_b = dt(scale_b sum_k keep_b x16[t, k] A_b[r, k])     (fp32 sums)
  *   x    [n_tok, width] F32 or dt (ldx);  a  dt [n_branch rank, width] (lda): the branches' lora_A
- *   x16  dt [n_tok, width] (ldx16), may be NULL;  u  dt [n_tok, n_branch rank] (ldu)
+ *   x16  dt [n_tok, width] (ldx16), may be NULL;  u  dt [n_tok, u_cols] (ldu): the branches' n_branch rank
+ *        columns, then (u_cols larger) a 1 and zeros, as decik_qkv_proj_gemm takes them with u_cols 64
  * Replaces lora_A(dropout(x)) of the reference's LoRA branches (solution/attn.py:217-228) without its
  * masks and masked copies. Backward, from du dt [n_tok, n_branch rank] (ld_du) and the forward's x16:
  *   dx = addend + sum_b scale_b keep_b (du_b A_b)      fp32 [n_tok, width]
@@ -486,8 +496,8 @@ DECIK_API int decik_dropout(const void* x, int x_dtype, const void* residual, vo
  * width % 8 == 0; rank % 8 == 0, the branches' ranks rounded up to 16 together <= 64; rows and
  * pointers 16-byte aligned. */
 DECIK_API int decik_lora_down_dropout(const void* x, int x_dtype, int64_t ldx, const void* a, int64_t lda, void* x16,
-                                      int64_t ldx16, void* u, int64_t ldu, int64_t n_tok, int width, int rank,
-                                      int n_branch, double p0, double p1, const int64_t* rng, int64_t stream_id,
+                                      int64_t ldx16, void* u, int64_t ldu, int u_cols, int64_t n_tok, int width,
+                                      int rank, int n_branch, double p0, double p1, const int64_t* rng, int64_t stream_id,
                                       int dtype, void* stream);
 DECIK_API int64_t decik_lora_down_dropout_bwd_workspace(int64_t n_tok, int width, int rank, int n_branch);
 DECIK_API int decik_lora_down_dropout_bwd(const void* du, int64_t ld_du, const void* x16, int64_t ldx, const void* a,

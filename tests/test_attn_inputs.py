@@ -106,7 +106,7 @@ def _refused(rc, text, code=1):
 def test_dropout_refuses_p(p):
     lib = _lib.lib()
     _refused(lib.decik_dropout(P, 1, None, P, 1, 8, p, P, 0, None), b"not in [0, 1]")
-    _refused(lib.decik_lora_down_dropout(P, 2, 64, P, 64, P, 64, P, 32, 4, 64, 16, 2, 0.1, p, P, 0, 1, None),
+    _refused(lib.decik_lora_down_dropout(P, 2, 64, P, 64, P, 64, P, 32, 32, 4, 64, 16, 2, 0.1, p, P, 0, 1, None),
              b"not in [0, 1]")
 
 
@@ -120,8 +120,8 @@ def test_dropout_refusals():
 
 def test_lora_refusals():
     lib = _lib.lib()
-    fwd = lambda x=P, xd=2, ldx=64, ldu=32, n=4, w=64, r=16, nb=2, dt=1: lib.decik_lora_down_dropout(
-        x, xd, ldx, P, 64, P, 64, P, ldu, n, w, r, nb, 0.1, 0.1, P, 0, dt, None)
+    fwd = lambda x=P, xd=2, ldx=64, ldu=64, uc=32, n=4, w=64, r=16, nb=2, dt=1: lib.decik_lora_down_dropout(
+        x, xd, ldx, P, 64, P, 64, P, ldu, uc, n, w, r, nb, 0.1, 0.1, P, 0, dt, None)
     _refused(fwd(w=60), b"width 60")
     _refused(fwd(n=-1), b"T=-1")
     _refused(fwd(r=12), b"rank 12", 3)
@@ -131,6 +131,8 @@ def test_lora_refusals():
     _refused(fwd(xd=0), b"x of dtype 0")
     _refused(fwd(ldx=56), b"strides shorter")
     _refused(fwd(ldu=24), b"strides shorter")
+    _refused(fwd(uc=24), b"u_cols 24")
+    _refused(fwd(uc=36), b"u_cols 36")
     _refused(fwd(x=ODD), b"alignment")
     _refused(fwd(ldx=66), b"alignment")
     assert fwd(n=0) == 0
