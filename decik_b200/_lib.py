@@ -6,10 +6,14 @@ There is no fallback: if the library is missing or a call fails, a RuntimeError 
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 import threading
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libdecik_b200.so")
+
+BIND_PATH = os.path.join(os.path.dirname(LIB_PATH), "_attn_inputs.so")
 
 F16, BF16, F32 = 0, 1, 2
 
@@ -156,6 +160,31 @@ def lib() -> ctypes.CDLL:
                     fn.argtypes = args
                 _lib = handle
     return _lib
+
+
+_bind = None
+
+
+def bind():
+    """The torch binding of the attention-input operators (csrc/host/attn_inputs.cpp; loads it on first
+    use)."""
+    global _bind
+    if _bind is None:
+        lib()  # the library it calls
+        with _lock:
+            if _bind is None:
+                import torch
+
+                if not os.path.exists(BIND_PATH):
+                    raise RuntimeError(f"decik_b200: {BIND_PATH} is not built; run `python -m decik_b200.build`")
+                loader = importlib.machinery.ExtensionFileLoader("_attn_inputs", BIND_PATH)
+                module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_attn_inputs", loader))
+                loader.exec_module(module)
+                if module.torch_version != torch.__version__:
+                    raise RuntimeError(f"decik_b200: {BIND_PATH} was built against torch {module.torch_version}, this is "
+                                       f"{torch.__version__}; run `python -m decik_b200.build`")
+                _bind = module
+    return _bind
 
 
 def check(rc: int, what: str) -> None:

@@ -231,74 +231,14 @@ def lora_input_grad(g_q, g_v, bits_q, bits_v, scale_q: float, scale_v: float):
 # ------------------------------------------------------------------------------------------------
 # norms of the query and key heads, rotation by positions of several axes
 # ------------------------------------------------------------------------------------------------
-_NONE3 = Tensor3(None, 0, 0)
-
-
-def _device(what: str, *ts: torch.Tensor | None) -> int:
-    """The index of the one CUDA device that all tensors are on (the first is never None)."""
-    dev = ts[0].get_device()
-    for t in ts:
-        if t is not None and t.get_device() != dev:
-            dev = -1
-    if dev < 0:
-        raise RuntimeError(f"decik_b200 {what}: tensors must be on one CUDA device (no CPU fallback)")
-    return dev
-
-
-def _launch(what: str, launches: int, dev: int, fn, *args) -> None:
-    """fn(*args, stream) on device ``dev``, on its current stream, timed while a recorder is installed."""
-    if dev != torch.cuda.current_device():
-        with torch.cuda.device(dev):
-            return _launch(what, launches, dev, fn, *args)
-    stream = torch._C._cuda_getCurrentRawStream(dev)  # current_stream(dev).cuda_stream without its Python objects
+def _bound(what: str, launches: int, *args):
+    """A function of the torch binding (csrc/host/attn_inputs.cpp), which checks its tensors, allocates
+    the results and enqueues on their device's current stream; timed while a recorder is installed."""
+    fn = getattr(_lib.bind(), what)
     if _timer is None:
-        rc = fn(*args, stream)
-    else:
-        with _timed(what, launches):
-            rc = fn(*args, stream)
-    if rc != 0:
-        _lib.check(rc, what)
-
-
-def _view3(what: str, t: torch.Tensor, swap: bool = False) -> Tensor3:
-    """A [T, H, D] view (with ``swap`` [H, T, D]) for the C ABI; the stride of a dimension of one element
-    does not matter."""
-    (a, b, d), (sa, sb, sd) = t.shape, t.stride()
-    if sd != 1 and d > 1:
-        raise RuntimeError(f"decik_b200 {what}: [T, H, D] views need contiguous D")
-    sa, sb = sa if a > 1 else 0, sb if b > 1 else 0
-    return Tensor3(t.data_ptr(), sb, sa) if swap else Tensor3(t.data_ptr(), sa, sb)
-
-
-def _ld(t: torch.Tensor) -> int:
-    """The row stride of a 2-D tensor; of a single row its width."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
-def _heads(what: str, q, k, q_lora, q_weight, k_weight):
-    """The checks of [T, H, D] query and key views; (T, Hq, Hk, D, q, k, q_lora views)."""
-    qs, ks = q.shape, k.shape
-    if len(qs) != 3 or len(ks) != 3 or qs[0] != ks[0] or qs[2] != ks[2] or q.dtype != k.dtype:
-        raise RuntimeError(f"decik_b200 {what}: q [T, Hq, D] and k [T, Hk, D] of one dtype")
-    if q_lora is not None and (q_lora.shape != qs or q_lora.dtype != q.dtype):
-        raise RuntimeError(f"decik_b200 {what}: q_lora must be like q")
-    if q_weight is not None or k_weight is not None:
-        if q_weight is None or k_weight is None:
-            raise RuntimeError(f"decik_b200 {what}: norm weights for both queries and keys, or for neither")
-        if not (q_weight.shape == k_weight.shape == qs[2:] and q_weight.dtype == k_weight.dtype
-                and q_weight.is_contiguous() and k_weight.is_contiguous()):
-            raise RuntimeError(f"decik_b200 {what}: norm weights must be contiguous [head_dim] of one dtype")
-    return (qs[0], qs[1], ks[1], qs[2], _view3(what, q), _view3(what, k),
-            _NONE3 if q_lora is None else _view3(what, q_lora))
-
-
-def _tables(what: str, cos, sin, T: int) -> int:
-    """The checks of the cos / sin tables; their rotary_dim."""
-    shape = cos.shape
-    if not (len(shape) == 2 and shape == sin.shape and shape[0] == T and cos.dtype == sin.dtype == torch.float32
-            and cos.is_contiguous() and sin.is_contiguous()):
-        raise RuntimeError(f"decik_b200 {what}: cos and sin must be contiguous fp32 [T, rotary_dim]")
-    return shape[1]
+        return fn(*args)
+    with _timed(what, launches):
+        return fn(*args)
 
 
 @functools.lru_cache(maxsize=64)
@@ -318,44 +258,13 @@ def rope_axis_of(sections: tuple, interleaved: bool = False) -> bytes:
     return bytes(out)
 
 
-def _axes_args(what: str, positions, inv_freq, sections, interleaved, T: int):
-    """The checks of positions [axes, T], inv_freq [R / 2] and sections; (positions as they are passed,
-    C arguments, rotary_dim)."""
-    axis_of = rope_axis_of(tuple(sections), bool(interleaved))
-    if positions.dim() == 1:
-        positions = positions[None]
-    code = _MASK_CODES.get(positions.dtype, 2)
-    if code > 1 or positions.shape != (len(sections), T):
-        raise RuntimeError(f"decik_b200 {what}: positions must be int64 or int32 [axes, T], an axis for each section")
-    rows, step = positions.stride()
-    if (step != 1 and T > 1) or (rows < T and len(sections) > 1):
-        positions = positions.contiguous()
-        rows = T
-    if inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous() or inv_freq.shape != (len(axis_of),):
-        raise RuntimeError(f"decik_b200 {what}: inv_freq must be contiguous fp32 [sum(sections)]")
-    return positions, (_p(positions), code, rows, len(sections), _p(inv_freq), axis_of), 2 * len(axis_of)
-
-
-def _head_out(like: torch.Tensor, H: int, T: int, D: int):
-    """A new head-major [H, T, D] tensor and its view."""
-    out = like.new_empty((H, T, D))
-    return out, Tensor3(out.data_ptr(), D, T * D)
-
-
 def qk_norm_rope_fwd(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, eps: float,
                      cos: torch.Tensor, sin: torch.Tensor, q_lora: torch.Tensor | None = None):
     """RMSNorm of each query and key head (over its D values, with the weights [D]) and RoPE of its first
     cos.shape[1] dims in one pass (decik_qk_norm_rope_fwd). q, k: [T, H, D] views of fp16 / bf16 (D
     contiguous, 16-byte aligned strides); ``q_lora`` is added to q first; cos, sin fp32 [T, rotary_dim].
     Returns q [Hq, T, D], k [Hk, T, D] head-major, as rope_fwd does."""
-    what = "qk_norm_rope_fwd"
-    dev = _device(what, q, k, q_weight, k_weight, cos, sin, q_lora)
-    T, Hq, Hk, D, q3, k3, l3 = _heads(what, q, k, q_lora, q_weight, k_weight)
-    R = _tables(what, cos, sin, T)
-    (q_out, qo3), (k_out, ko3) = _head_out(q, Hq, T, D), _head_out(q, Hk, T, D)
-    _launch(what, 1, dev, _lib.lib().decik_qk_norm_rope_fwd, q3, l3, k3, q_weight.data_ptr(), k_weight.data_ptr(),
-            _dt(q_weight), eps, cos.data_ptr(), sin.data_ptr(), qo3, ko3, T, Hq, Hk, D, R, _dt(q))
-    return q_out, k_out
+    return _bound("qk_norm_rope_fwd", 1, q, k, q_weight, k_weight, eps, cos, sin, q_lora)
 
 
 def qk_norm_rope_bwd(grad_q: torch.Tensor, grad_k: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
@@ -364,16 +273,7 @@ def qk_norm_rope_bwd(grad_q: torch.Tensor, grad_k: torch.Tensor, q: torch.Tensor
     """The backward of qk_norm_rope_fwd from grad_q [Hq, T, D], grad_k [Hk, T, D] and the forward's inputs
     (decik_qk_norm_rope_bwd): dq [T, Hq, D] (of q and of q_lora), dk [T, Hk, D], and the weights'
     gradients fp32 [D]."""
-    what = "qk_norm_rope_bwd"
-    dev = _device(what, q, k, q_weight, k_weight, cos, sin, q_lora, grad_q, grad_k)
-    T, Hq, Hk, D, q3, k3, l3 = _heads(what, q, k, q_lora, q_weight, k_weight)
-    R = _tables(what, cos, sin, T)
-    gq3, gk3 = _head_grads(what, grad_q, grad_k, Hq, Hk, T, D, q.dtype)
-    dq, dk, dwq, dwk, ws = _head_outs(q, T, Hq, Hk, D, True)
-    _launch(what, 2, dev, _lib.lib().decik_qk_norm_rope_bwd, gq3, gk3, q3, l3, k3, q_weight.data_ptr(),
-            k_weight.data_ptr(), _dt(q_weight), eps, cos.data_ptr(), sin.data_ptr(), Tensor3(dq.data_ptr(), Hq * D, D),
-            Tensor3(dk.data_ptr(), Hk * D, D), dwq.data_ptr(), dwk.data_ptr(), T, Hq, Hk, D, R, _dt(q), ws.data_ptr())
-    return dq, dk, dwq, dwk
+    return _bound("qk_norm_rope_bwd", 2, grad_q, grad_k, q, k, q_weight, k_weight, eps, cos, sin, q_lora)
 
 
 def rope_axes_fwd(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, sections,
@@ -384,14 +284,9 @@ def rope_axes_fwd(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv
     int32 [axes, T] (or [T] for one axis), inv_freq fp32 [R / 2], ``sections`` the number of frequencies
     of each axis (rope_axis_of). With ``q_weight`` and ``k_weight`` each head is normed first, as in
     qk_norm_rope_fwd. q, k, q_lora and the results as there."""
-    what = "rope_axes_fwd"
-    dev = _device(what, q, k, positions, inv_freq, q_weight, k_weight, q_lora)
-    T, Hq, Hk, D, q3, k3, l3 = _heads(what, q, k, q_lora, q_weight, k_weight)
-    positions, axes, R = _axes_args(what, positions, inv_freq, sections, interleaved, T)
-    (q_out, qo3), (k_out, ko3) = _head_out(q, Hq, T, D), _head_out(q, Hk, T, D)
-    _launch(what, 1, dev, _lib.lib().decik_rope_axes_fwd, q3, l3, k3, _p(q_weight), _p(k_weight),
-            F32 if q_weight is None else _dt(q_weight), eps, *axes, qo3, ko3, T, Hq, Hk, D, R, _dt(q))
-    return q_out, k_out
+    sections = tuple(sections)
+    return _bound("rope_axes_fwd", 1, q, k, positions, inv_freq, rope_axis_of(sections, interleaved), len(sections),
+                  q_weight, k_weight, eps, q_lora)
 
 
 def rope_axes_bwd(grad_q: torch.Tensor, grad_k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
@@ -401,76 +296,29 @@ def rope_axes_bwd(grad_q: torch.Tensor, grad_k: torch.Tensor, positions: torch.T
     """The backward of rope_axes_fwd from grad_q [Hq, T, D], grad_k [Hk, T, D] (decik_rope_axes_bwd):
     (dq [T, Hq, D], dk [T, Hk, D]); with the norm weights (which need the forward's q, k and q_lora)
     also the weights' gradients fp32 [D]."""
-    what = "rope_axes_bwd"
-    dev = _device(what, grad_q, grad_k, positions, inv_freq, q, k, q_weight, k_weight, q_lora)
-    if grad_q.dim() != 3 or grad_k.dim() != 3:
-        raise RuntimeError(f"decik_b200 {what}: grad_q [Hq, T, D], grad_k [Hk, T, D]")
-    Hq, T, D = grad_q.shape
-    Hk = grad_k.shape[0]
-    norm = q_weight is not None or k_weight is not None
-    q3 = k3 = l3 = _NONE3
-    if norm:
-        if q is None or k is None:
-            raise RuntimeError(f"decik_b200 {what}: the backward of the norms needs the forward's q and k")
-        _, _, _, _, q3, k3, l3 = _heads(what, q, k, q_lora, q_weight, k_weight)
-        if q.shape != (T, Hq, D) or k.shape != (T, Hk, D):
-            raise RuntimeError(f"decik_b200 {what}: q and k must have the gradients' shapes")
-    positions, axes, R = _axes_args(what, positions, inv_freq, sections, interleaved, T)
-    gq3, gk3 = _head_grads(what, grad_q, grad_k, Hq, Hk, T, D, q.dtype if norm else grad_q.dtype)
-    dq, dk, dwq, dwk, ws = _head_outs(grad_q, T, Hq, Hk, D, norm)
-    _launch(what, 2 if norm else 1, dev, _lib.lib().decik_rope_axes_bwd, gq3, gk3, q3, l3, k3, _p(q_weight),
-            _p(k_weight), _dt(q_weight) if norm else F32, eps, *axes, Tensor3(dq.data_ptr(), Hq * D, D),
-            Tensor3(dk.data_ptr(), Hk * D, D), _p(dwq), _p(dwk), T, Hq, Hk, D, R, _dt(grad_q), _p(ws))
-    return (dq, dk, dwq, dwk) if norm else (dq, dk)
-
-
-def _head_grads(what, grad_q, grad_k, Hq, Hk, T, D, dtype):
-    if grad_q.shape != (Hq, T, D) or grad_k.shape != (Hk, T, D) or grad_q.dtype != dtype or grad_k.dtype != dtype:
-        raise RuntimeError(f"decik_b200 {what}: grad_q [Hq, T, D] and grad_k [Hk, T, D] of the inputs' dtype")
-    return _view3(what, grad_q, swap=True), _view3(what, grad_k, swap=True)
-
-
-def _head_outs(like, T, Hq, Hk, D, norm: bool):
-    dq, dk = like.new_empty((T, Hq, D)), like.new_empty((T, Hk, D))
-    if not norm:
-        return dq, dk, None, None, None
-    dwq, dwk = (like.new_empty((D,), dtype=torch.float32) for _ in range(2))
-    ws = like.new_empty((_lib.lib().decik_qk_norm_rope_bwd_workspace(D),), dtype=torch.uint8)
-    return dq, dk, dwq, dwk, ws
+    sections = tuple(sections)
+    return _bound("rope_axes_bwd", 1 if q_weight is None else 2, grad_q, grad_k, positions, inv_freq,
+                  rope_axis_of(sections, interleaved), len(sections), q, k, q_weight, k_weight, eps, q_lora)
 
 
 # ------------------------------------------------------------------------------------------------
 # dropout from a counter-based generator
 # ------------------------------------------------------------------------------------------------
-def _check_rng(what: str, rng: torch.Tensor) -> None:
-    if rng.dtype != torch.int64 or rng.shape != (2,) or not rng.is_contiguous():
-        raise RuntimeError(f"decik_b200 {what}: rng must be int64 [2] (seed, offset)")
-
-
 def dropout(x: torch.Tensor, p: float, rng: torch.Tensor, stream: int = 0, residual: torch.Tensor | None = None,
             out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """keep * scale * x, or residual + keep * scale * x, with the mask of (rng, stream) over x's values in
     row-major order (decik_dropout; no mask is stored). ``rng``: int64 [2] on x's device, (seed,
     offset); two streams of one rng are independent masks. The result has the residual's dtype, else
     ``out_dtype`` or x's. The backward is the same call on the gradient, with out_dtype = x's dtype."""
-    dev = _device("dropout", x, rng, residual)
-    _check_rng("dropout", rng)
-    if residual is not None and (residual.shape != x.shape or out_dtype not in (None, residual.dtype)):
-        raise RuntimeError("decik_b200 dropout: residual must be like x, and gives the result its dtype")
-    x = x.contiguous()
-    res = None if residual is None else residual.contiguous()
-    out = x.new_empty(x.shape, dtype=residual.dtype if residual is not None else out_dtype or x.dtype)
-    _launch("dropout", 1, dev, _lib.lib().decik_dropout, x.data_ptr(), _dt(x), _p(res), out.data_ptr(), _dt(out),
-            x.numel(), p, rng.data_ptr(), stream)
-    return out
+    return _bound("dropout", 1, x, p, rng, stream, residual, out_dtype)
 
 
-def _branches(what: str, a: torch.Tensor, p, width: int):
-    """(rank, branches, p of each) of a [branches * rank, width] and p, a number or one for each branch."""
+def _branch_ps(what: str, p):
+    """(branches, p of the first, p of the second) of a number or a tuple."""
     ps = tuple(p) if isinstance(p, (tuple, list)) else (p,)
-    if a.dim() != 2 or a.shape[1] != width or a.stride(1) != 1 or not 1 <= len(ps) <= 2 or a.shape[0] % len(ps):
-        raise RuntimeError(f"decik_b200 {what}: a must be [branches * rank, width] with a p for each of 1 or 2 branches")
-    return a.shape[0] // len(ps), len(ps), ps if len(ps) == 2 else (ps[0], 0.0)
+    if not 1 <= len(ps) <= 2:
+        raise RuntimeError(f"decik_b200 {what}: a p for each of 1 or 2 branches")
+    return (2, *ps) if len(ps) == 2 else (1, ps[0], 0.0)
 
 
 def lora_down_dropout(x: torch.Tensor, a: torch.Tensor, p, rng: torch.Tensor, stream: int = 0,
@@ -481,23 +329,7 @@ def lora_down_dropout(x: torch.Tensor, a: torch.Tensor, p, rng: torch.Tensor, st
     Returns x16 = x in a's dtype (x itself where it has it) and u [T, branches * rank] =
     scale_b (keep_b x16) A_b^T; with ``u_cols`` (64 for qkv_proj_gemm) u has that many columns, a 1 and
     zeros behind the branches'."""
-    what = "lora_down_dropout"
-    dev = _device(what, x, a, rng)
-    _check_rng(what, rng)
-    if x.dim() != 2 or x.dtype not in (torch.float32, a.dtype):
-        raise RuntimeError(f"decik_b200 {what}: x must be [T, width], fp32 or of a's dtype")
-    if x.stride(1) != 1:
-        x = x.contiguous()
-    T, W = x.shape
-    rank, nb, ps = _branches(what, a, p, W)
-    x16 = x if x.dtype == a.dtype else a.new_empty((T, W))
-    u_cols = nb * rank if u_cols is None else u_cols
-    u = a.new_empty((T, u_cols))
-    _launch(what, 1, dev, _lib.lib().decik_lora_down_dropout, x.data_ptr(), _dt(x), _ld(x), a.data_ptr(), _ld(a),
-            None if x16 is x else x16.data_ptr(), W, u.data_ptr(), u_cols, u_cols, T, W, rank, nb, *ps,
-            rng.data_ptr(),
-            stream, _dt(a))
-    return x16, u
+    return _bound("lora_down_dropout", 1, x, a, *_branch_ps("lora_down_dropout", p), rng, stream, u_cols or 0)
 
 
 def lora_down_dropout_bwd(du: torch.Tensor, x16: torch.Tensor, a: torch.Tensor, p, rng: torch.Tensor,
@@ -506,26 +338,8 @@ def lora_down_dropout_bwd(du: torch.Tensor, x16: torch.Tensor, a: torch.Tensor, 
     values it had in the forward) and stream (decik_lora_down_dropout_bwd): dx fp32 [T, W] =
     addend + sum_b scale_b keep_b (du_b A_b) and da fp32 [branches * rank, W]. ``out``: a buffer for dx
     (it may be ``addend``)."""
-    what = "lora_down_dropout_bwd"
-    dev = _device(what, x16, du, a, rng, addend, out)
-    _check_rng(what, rng)
-    if x16.dim() != 2 or x16.stride(1) != 1 or x16.dtype != a.dtype:
-        raise RuntimeError(f"decik_b200 {what}: x16 must be [T, width] of a's dtype with contiguous rows")
-    T, W = x16.shape
-    rank, nb, ps = _branches(what, a, p, W)
-    if du.shape != (T, nb * rank) or du.dtype != a.dtype or du.stride(1) != 1:
-        raise RuntimeError(f"decik_b200 {what}: du must be [T, branches * rank] of a's dtype with contiguous rows")
-    for t in (addend, out):
-        if t is not None and (t.shape != (T, W) or t.dtype != torch.float32 or t.stride(1) != 1):
-            raise RuntimeError(f"decik_b200 {what}: addend and out must be fp32 [T, width] with contiguous rows")
-    lib = _lib.lib()
-    dx = x16.new_empty((T, W), dtype=torch.float32) if out is None else out
-    da = x16.new_empty((nb * rank, W), dtype=torch.float32)
-    ws = x16.new_empty((lib.decik_lora_down_dropout_bwd_workspace(T, W, rank, nb),), dtype=torch.uint8)
-    _launch(what, 2, dev, lib.decik_lora_down_dropout_bwd, du.data_ptr(), _ld(du), x16.data_ptr(), _ld(x16),
-            a.data_ptr(), _ld(a), _p(addend), 0 if addend is None else _ld(addend), dx.data_ptr(), _ld(dx),
-            da.data_ptr(), T, W, rank, nb, *ps, rng.data_ptr(), stream, _dt(a), ws.data_ptr())
-    return dx, da
+    return _bound("lora_down_dropout_bwd", 2, du, x16, a, *_branch_ps("lora_down_dropout_bwd", p), rng, stream, addend,
+                  out)
 
 
 # ------------------------------------------------------------------------------------------------
