@@ -90,147 +90,136 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
 // ------------------------------------------------------------------------------------------------
 // forward
 // ------------------------------------------------------------------------------------------------
-// A CTA takes 16 MT rows; its warps share out the width in blocks of 32 columns and their partial
-// sums meet in shared memory. In a block, lane 4 g + c holds the 8 columns from 8 c of rows g and g + 8
-// (of each 16): 32 bytes of x in one go, one call of the generator per row and branch, and, because
-// the order of a sum's terms is free, an operand fragment of mma.sync m16n8k16 without any exchange:
-// the instruction's columns 2 c, 2 c + 1 and 2 c + 8, 2 c + 9 of step s are the lane's pairs 2 s and
-// 2 s + 1. lora_A's rows, read the same way (16 bytes of row g), are the other operand.
-// The next block's bytes are on their way through cp.async, into the warp's own ring, while one is
-// computed.
-template <typename X, typename T, int NB, int NTB, int MT>
+// A CTA takes 16 rows; its 8 warps share out the width in blocks of 32 columns and their partial sums meet
+// in shared memory. In a block, lane 4 g + c holds the 8 columns from 8 c of rows g and g + 8: one call of
+// the generator per row and branch, and, because the order of a sum's terms is free, an operand fragment
+// of mma.sync m16n8k16 without any exchange: the instruction's columns 2 c, 2 c + 1 and 2 c + 8, 2 c + 9
+// of step s are the lane's pairs 2 s and 2 s + 1. lora_A's rows, read the same way (16 bytes of row g),
+// are the other operand. The next kStages - 1 blocks' bytes are on their way through cp.async, into the
+// warp's own ring, while one is computed.
+constexpr int kWarps = 8, kStages = 3;
+
+template <typename X, int NT>  // NT: n8 tiles of u's columns
 struct DownTile {
-  static constexpr int kXPieces = sizeof(X) / 2;                       // 16-byte pieces of 8 columns
-  static constexpr int kPieces = MT * 2 * kXPieces + NB * NTB;         // of a lane, per block
-  static constexpr int kStage = kPieces * 512;                         // bytes of a warp's stage
-  static constexpr int kLd = 8 * NB * NTB + 4;                         // row of the partial sums
-  static constexpr int smem(int warps) {
-    const int ring = 2 * warps * kStage, red = warps * 16 * kLd * 4;
-    return ring > red ? ring : red;
-  }
+  static constexpr int kXPieces = sizeof(X) / 2;                // 16-byte pieces of 8 columns
+  static constexpr int kStage = (2 * kXPieces + NT) * 512;      // bytes of a warp's stage
+  static constexpr int kLd = 8 * NT + 4;                        // row of the partial sums
+  static constexpr int kRing = kStages * kWarps * kStage, kRed = kWarps * 16 * kLd * 4;
+  static constexpr int kSmem = kRing > kRed ? kRing : kRed;
 };
 
-template <typename X, typename T, int NB, int NTB, int MT, int WARPS>
-__global__ void __launch_bounds__(32 * WARPS, NB * NTB <= 4 ? (WARPS == 4 ? 5 : 2) : 8 / WARPS)
+template <typename X, typename T, int NB, int NTB>
+__global__ void __launch_bounds__(32 * kWarps, 2)
 down_kernel(const X* __restrict__ x, int64_t ldx, const T* __restrict__ a, int64_t lda, T* __restrict__ x16,
             int64_t ldx16, T* __restrict__ u, int64_t ldu, int u_cols, int64_t n_tok, int width, int rank, Drop d,
             const int64_t* __restrict__ rng, int64_t stream_id) {
-  using Tile = DownTile<X, T, NB, NTB, MT>;
-  constexpr int NT = NB * NTB, XP = Tile::kXPieces, LD = Tile::kLd;   // NT: n8 tiles of u's columns
+  constexpr int NT = NB * NTB;
+  using Tile = DownTile<X, NT>;
+  constexpr int XP = Tile::kXPieces, LD = Tile::kLd, kXBytes = 2 * XP * 512;
   extern __shared__ __align__(16) unsigned char smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * (16 * MT);
-  const philox::Key key = philox::make_key(rng);
-  philox::Stream ctr[NB];
-#pragma unroll
-  for (int b = 0; b < NB; ++b) ctr[b] = philox::make_stream(rng, stream_id + b);
-  float acc[MT][NT][4];
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[m][n][e] = 0.f;
-  unsigned char* const ring = smem + warp * (2 * Tile::kStage);  // x, then A: a lane's own piece n at 512 n + 16 lane
-  constexpr int kXBytes = 2 * MT * XP * 512;
-  const int rows = n_tok - t0 < 16 * MT ? static_cast<int>(n_tok - t0) : 16 * MT;
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * 16;
+  const int rows = n_tok - t0 < 16 ? static_cast<int>(n_tok - t0) : 16;
   // The pieces of the block with its columns at k0, zeros behind the width. Rows that are not there (of x
   // behind the last token, of A behind the rank) are others read again: what comes of them is not stored.
-  constexpr int XN = 2 * MT * XP, XR = XP == 2 ? 4 : 8, XE = 16 / sizeof(X);  // a copy's pieces, rows, elements
+  constexpr int XN = 2 * XP, XR = XP == 2 ? 4 : 8, XE = 16 / sizeof(X);  // a copy's pieces, rows, elements
   const int xr = XP == 2 ? lane >> 3 : g, xc = XP == 2 ? 4 * (lane & 7) : 8 * c;  // the lane's row and column
   const X* xp[XN];
   const T* ap[NT];
 #pragma unroll
   for (int i = 0; i < XN; ++i) xp[i] = x + (t0 + (XR * i + xr < rows ? XR * i + xr : 0)) * ldx;
 #pragma unroll
-  for (int n = 0; n < NT; ++n) ap[n] = a + static_cast<int64_t>(8 * (n % NTB) < rank ? n / NTB * rank + 8 * (n % NTB) + g : 0) * lda;
+  for (int n = 0; n < NT; ++n)
+    ap[n] = a + static_cast<int64_t>(8 * (n % NTB) < rank ? n / NTB * rank + 8 * (n % NTB) + g : 0) * lda;
+  unsigned char* const ring = smem + warp * (kStages * Tile::kStage);  // x, then A: a lane's own piece n at 512 n + 16 lane
+  const uint32_t ring_at = ptx::smem_u32(ring);
   auto issue = [&](int stage, int k0) {
-    const uint32_t dst = ptx::smem_u32(ring) + stage * Tile::kStage;
-    const bool xin = k0 + xc < width, ain = k0 + 8 * c < width;
-    const int xk = xin ? k0 + xc : width - XE, ak = ain ? k0 + 8 * c : width - 8;
+    if (k0 < width) {
+      const uint32_t dst = ring_at + stage * Tile::kStage;
+      const bool xin = k0 + xc < width, ain = k0 + 8 * c < width;
+      const int xk = xin ? k0 + xc : width - XE, ak = ain ? k0 + 8 * c : width - 8;
 #pragma unroll
-    for (int i = 0; i < XN; ++i)
-      ptx::cp_async16(dst + (XP == 2 ? block_at(XR * i + xr, lane & 7) : i * 512 + lane * 16), xp[i] + xk, xin);
+      for (int i = 0; i < XN; ++i)
+        ptx::cp_async16(dst + (XP == 2 ? block_at(XR * i + xr, lane & 7) : i * 512 + lane * 16), xp[i] + xk, xin);
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-      ptx::cp_async16(dst + kXBytes + n * 512 + lane * 16, ap[n] + ak, ain);
+      for (int n = 0; n < NT; ++n) ptx::cp_async16(dst + kXBytes + n * 512 + lane * 16, ap[n] + ak, ain);
+    }
+    ptx::cp_async_commit();
   };
-  int stage = 0;
-  const int step = 32 * WARPS;
+  constexpr int kStep = 32 * kWarps;
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) issue(s, 32 * warp + s * kStep);
+  const philox::Key key = philox::make_key(rng);
+  philox::Stream ctr[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) ctr[b] = philox::make_stream(rng, stream_id + b);
+  float acc[NT][4] = {};
   T* const x16p = x16 + (t0 + g) * ldx16;
   const unsigned long long group0 = static_cast<unsigned long long>(t0 + g) * (width / 8);
-  if (32 * warp < width) issue(0, 32 * warp);
-  ptx::cp_async_commit();
-  for (int k = 32 * warp + 8 * c; k - 8 * c < width; k += step, stage ^= 1) {
-    __syncwarp();  // the other stage has been read
-    if (k - 8 * c + step < width) issue(stage ^ 1, k - 8 * c + step);
-    ptx::cp_async_commit();
-    ptx::cp_async_wait<1>();
-    __syncwarp();
+  int stage = 0;
+  for (int k0 = 32 * warp; k0 < width; k0 += kStep) {
+    const int k = k0 + 8 * c;
+    ptx::cp_async_wait<kStages - 2>();
+    __syncwarp();  // this stage has landed for every lane, and the one issued next has been read by all
+    issue(stage == 0 ? kStages - 1 : stage - 1, k0 + (kStages - 1) * kStep);
     const unsigned char* const got = ring + stage * Tile::kStage;
-    uint4 av[NT];
+    uint4 av[NT], xv[2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) av[n] = *reinterpret_cast<const uint4*>(got + kXBytes + n * 512 + lane * 16);
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      uint4 xv[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if constexpr (XP == 1) {
-          xv[h] = *reinterpret_cast<const uint4*>(got + (2 * m + h) * 512 + lane * 16);
-        } else {
-          float f[8];
-          block_read(got, 16 * m + 8 * h + g, c, f);
-          xv[h] = pack8<T>(f);
-        }
-        if (x16 != nullptr && k < width && 16 * m + 8 * h + g < rows) stg16(x16p + (16 * m + 8 * h) * ldx16 + k, xv[h]);
+    for (int h = 0; h < 2; ++h) {
+      if constexpr (XP == 1) {
+        xv[h] = *reinterpret_cast<const uint4*>(got + h * 512 + lane * 16);
+      } else {
+        float f[8];
+        block_read(got, 8 * h + g, c, f);
+        xv[h] = pack8<T>(f);
       }
+      if (x16 != nullptr && k < width && 8 * h + g < rows) stg16(x16p + 8 * h * ldx16 + k, xv[h]);
+    }
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        uint32_t lo[4], hi[4];
-        const unsigned long long group = group0 + static_cast<unsigned long long>(2 * m * width + k / 8);
-        mask8(philox::words(key, ctr[b], group), xv[0], d.cut[b], d, lo);
-        mask8(philox::words(key, ctr[b], group + static_cast<unsigned long long>(width)), xv[1], d.cut[b], d, hi);
-        const uint32_t f0[4] = {lo[0], hi[0], lo[1], hi[1]}, f1[4] = {lo[2], hi[2], lo[3], hi[3]};
+    for (int b = 0; b < NB; ++b) {
+      uint32_t lo[4], hi[4];
+      const unsigned long long group = group0 + static_cast<unsigned long long>(k / 8);
+      mask8(philox::words(key, ctr[b], group), xv[0], d.cut[b], d, lo);
+      mask8(philox::words(key, ctr[b], group + static_cast<unsigned long long>(width)), xv[1], d.cut[b], d, hi);
+      const uint32_t f0[4] = {lo[0], hi[0], lo[1], hi[1]}, f1[4] = {lo[2], hi[2], lo[3], hi[3]};
 #pragma unroll
-        for (int n = b * NTB; n < (b + 1) * NTB; ++n) {
-          ptx::mma16816<T>(acc[m][n], f0, av[n].x, av[n].y);
-          ptx::mma16816<T>(acc[m][n], f1, av[n].z, av[n].w);
-        }
+      for (int n = b * NTB; n < (b + 1) * NTB; ++n) {
+        ptx::mma16816<T>(acc[n], f0, av[n].x, av[n].y);
+        ptx::mma16816<T>(acc[n], f1, av[n].z, av[n].w);
       }
     }
+    stage = stage + 1 == kStages ? 0 : stage + 1;
   }
-  // the warps' sums in shared memory, over the ring
+  // the warps' sums in shared memory, over the rings
   ptx::cp_async_wait<0>();
-  float* const red = reinterpret_cast<float*>(smem);  // [WARPS][16][LD]
+  __syncthreads();
+  float* const red = reinterpret_cast<float*>(smem);  // [kWarps][16][LD]
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    __syncthreads();
+  for (int n = 0; n < NT; ++n) {
+    float* const p = red + (warp * 16 + g) * LD + 8 * n + 2 * c;
+    *reinterpret_cast<float2*>(p) = make_float2(acc[n][0], acc[n][1]);
+    *reinterpret_cast<float2*>(p + 8 * LD) = make_float2(acc[n][2], acc[n][3]);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 16 * 4 * NT; i += 32 * kWarps) {  // a pair of u's columns
+    const int row = i / (4 * NT), col = 2 * (i % (4 * NT)), b = col / (8 * NTB), r = col % (8 * NTB);
+    if (row >= rows || r >= rank) continue;
+    float2 s = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      float* const p = red + (warp * 16 + g) * LD + 8 * n + 2 * c;
-      *reinterpret_cast<float2*>(p) = make_float2(acc[m][n][0], acc[m][n][1]);
-      *reinterpret_cast<float2*>(p + 8 * LD) = make_float2(acc[m][n][2], acc[m][n][3]);
+    for (int w = 0; w < kWarps; ++w) {
+      const float2 v = *reinterpret_cast<const float2*>(red + (w * 16 + row) * LD + col);
+      s.x += v.x;
+      s.y += v.y;
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < 16 * 4 * NT; i += 32 * WARPS) {  // a pair of u's columns
-      const int row = i / (4 * NT), col = 2 * (i % (4 * NT)), b = col / (8 * NTB), r = col % (8 * NTB);
-      const int64_t t = t0 + 16 * m + row;
-      if (t >= n_tok || r >= rank) continue;
-      float2 s = make_float2(0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
-        const float2 v = *reinterpret_cast<const float2*>(red + (w * 16 + row) * LD + col);
-        s.x += v.x;
-        s.y += v.y;
-      }
-      const float scale = NB == 2 && b == 1 ? d.scale[1] : d.scale[0];
-      *reinterpret_cast<uint32_t*>(u + t * ldu + b * rank + r) = scale == 0.f ? 0u : Dt<T>::pack2(s.x * scale, s.y * scale);
-    }
+    const float scale = NB == 2 && b == 1 ? d.scale[1] : d.scale[0];
+    *reinterpret_cast<uint32_t*>(u + (t0 + row) * ldu + b * rank + r) =
+        scale == 0.f ? 0u : Dt<T>::pack2(s.x * scale, s.y * scale);
   }
   // the columns behind the branches': a 1 (it multiplies the bias in the projection's extra K block), zeros
   const int n_u = NB * rank, more = (u_cols - n_u) / 2;
-  for (int i = threadIdx.x; i < rows * more; i += 32 * WARPS)
+  for (int i = threadIdx.x; i < rows * more; i += 32 * kWarps)
     *reinterpret_cast<uint32_t*>(u + (t0 + i / more) * ldu + n_u + 2 * (i % more)) =
         i % more == 0 ? Dt<T>::pack2(1.f, 0.f) : 0u;
 }
@@ -515,23 +504,16 @@ struct DownArgs {
   cudaStream_t s;
 };
 
-template <typename X, typename T, int NB, int NTB, int MT, int WARPS>
-int launch_down_m(const DownArgs& p) {
+template <typename X, typename T, int NB, int NTB>
+int launch_down_t(const DownArgs& p) {
   static std::atomic<unsigned long long> done{0};
-  constexpr int smem = DownTile<X, T, NB, NTB, MT>::smem(WARPS);
-  auto kernel = down_kernel<X, T, NB, NTB, MT, WARPS>;
+  constexpr int smem = DownTile<X, NB * NTB>::kSmem;
+  auto kernel = down_kernel<X, T, NB, NTB>;
   if (int rc = ensure_dyn_smem(kernel, smem, done, "lora_down_dropout")) return rc;
-  kernel<<<static_cast<unsigned>((p.n_tok + 16 * MT - 1) / (16 * MT)), 32 * WARPS, smem, p.s>>>(
+  kernel<<<static_cast<unsigned>((p.n_tok + 15) / 16), 32 * kWarps, smem, p.s>>>(
       static_cast<const X*>(p.x), p.ldx, static_cast<const T*>(p.a), p.lda, static_cast<T*>(p.x16), p.ldx16,
       static_cast<T*>(p.u), p.ldu, p.u_cols, p.n_tok, p.width, p.rank, p.d, p.rng, p.stream_id);
   return check_launch("lora_down_dropout");
-}
-
-// Few rows: the width over 8 warps, many: over 4.
-template <typename X, typename T, int NB, int NTB>
-int launch_down_t(const DownArgs& p) {
-  return p.n_tok <= 32 * static_cast<int64_t>(sm_count()) ? launch_down_m<X, T, NB, NTB, 1, 8>(p)
-                                                          : launch_down_m<X, T, NB, NTB, 1, 4>(p);
 }
 
 template <typename X, typename T>
