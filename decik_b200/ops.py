@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import operator
 
 import torch
 
@@ -241,11 +242,18 @@ def _bound(what: str, launches: int, *args):
         return fn(*args)
 
 
-@functools.lru_cache(maxsize=64)
-def rope_axis_of(sections: tuple, interleaved: bool = False) -> bytes:
+def rope_axis_of(sections, interleaved: bool = False) -> bytes:
     """The axis of each rotary frequency: ``sections[a]`` frequencies of axis a, one block after the
     other, or ``interleaved``: the axes in turn (0, 1, 2, 0, ...) while they have some left."""
-    if not 1 <= len(sections) <= 4 or any(int(n) != n or n < 0 for n in sections):
+    try:
+        return _axis_of(tuple(map(operator.index, sections)), bool(interleaved))
+    except TypeError:
+        raise RuntimeError("decik_b200 rope_axes: sections must be 1 to 4 counts of frequencies") from None
+
+
+@functools.lru_cache(maxsize=64)
+def _axis_of(sections: tuple, interleaved: bool) -> bytes:
+    if not 1 <= len(sections) <= 4 or any(n < 0 for n in sections):
         raise RuntimeError("decik_b200 rope_axes: sections must be 1 to 4 counts of frequencies")
     if not interleaved:
         return bytes(a for a, n in enumerate(sections) for _ in range(n))
@@ -282,9 +290,8 @@ def rope_axes_fwd(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv
     """RoPE by positions of several axes (decik_rope_axes_fwd): the angle of frequency j is
     positions[axis of j] * inv_freq[j], computed in the kernel (no cos / sin tables). positions int64 or
     int32 [axes, T] (or [T] for one axis), inv_freq fp32 [R / 2], ``sections`` the number of frequencies
-    of each axis (rope_axis_of). With ``q_weight`` and ``k_weight`` each head is normed first, as in
+    of each axis (rope_axis_of), R / 2 = their sum a multiple of 8. With ``q_weight`` and ``k_weight`` each head is normed first, as in
     qk_norm_rope_fwd. q, k, q_lora and the results as there."""
-    sections = tuple(sections)
     return _bound("rope_axes_fwd", 1, q, k, positions, inv_freq, rope_axis_of(sections, interleaved), len(sections),
                   q_weight, k_weight, eps, q_lora)
 
@@ -296,7 +303,6 @@ def rope_axes_bwd(grad_q: torch.Tensor, grad_k: torch.Tensor, positions: torch.T
     """The backward of rope_axes_fwd from grad_q [Hq, T, D], grad_k [Hk, T, D] (decik_rope_axes_bwd):
     (dq [T, Hq, D], dk [T, Hk, D]); with the norm weights (which need the forward's q, k and q_lora)
     also the weights' gradients fp32 [D]."""
-    sections = tuple(sections)
     return _bound("rope_axes_bwd", 1 if q_weight is None else 2, grad_q, grad_k, positions, inv_freq,
                   rope_axis_of(sections, interleaved), len(sections), q, k, q_weight, k_weight, eps, q_lora)
 

@@ -12,9 +12,9 @@
 - ``SKC_ATTN``        Qwen2Attention forward: LoRA + RoPE + varlen attention (attn.py);
                       ``SKC_LORA_RECOMPUTE``; ``SKC_FUSED_BLOCK`` (this build's addition: LoRA
                       without dropout runs as one fused projection + attention node)
-- ``SKC_COUNTER_DROPOUT=<seed>`` (this build's addition, off unless set): dropout on the packed path from
-                      a counter-based generator with no stored masks; LoRA with dropout then takes the
-                      fused node too (dropout.py; ``dropout.use_counter_dropout``)
+- ``SKC_COUNTER_DROPOUT=<seed>`` (this build's addition, off where unset or 0): dropout on the packed path
+                      from a counter-based generator with no stored masks; LoRA with dropout then takes
+                      the fused node too (dropout.py; ``dropout.use_counter_dropout``)
 The reference's head, embedding and warm-up patches are outside this build's scope.
 Patches whose third-party library is not installed (bitsandbytes, peft) are skipped with a
 warning; an eligible input never falls back to a CPU or per-row path.
@@ -37,8 +37,9 @@ def apply(linear4bit_cls=None, lora_classes=None):
         except ImportError as e:
             warnings.warn(f"decik_b200.solution.apply: {what} not patched ({e})")
 
-    if os.environ.get("SKC_COUNTER_DROPOUT"):
-        dropout.use_counter_dropout(int(os.environ["SKC_COUNTER_DROPOUT"]))
+    seed = int(os.environ.get("SKC_COUNTER_DROPOUT") or 0)
+    if seed:
+        dropout.use_counter_dropout(seed)
     if _enabled("NF4"):
         _try(nf4.patch, "Linear4bit", linear4bit_cls)
     if _enabled("RMSNORM"):

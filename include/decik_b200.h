@@ -477,7 +477,8 @@ DECIK_API int decik_mlp_down_grad(const void* grad, int64_t ldg, const void* w_d
  *
  * decik_dropout: out = keep scale x, or with residual (out's type, may be NULL) residual + keep scale x,
  * over n values; one rounding, to out's type. x, out: F16, BF16 or F32 each, of any alignment; out
- * may be x or residual. The backward of the dropout is the same call on the gradient. */
+ * may be residual, or x where their types are the same. The backward of the dropout is the same call on
+ * the gradient. */
 DECIK_API int decik_dropout(const void* x, int x_dtype, const void* residual, void* out, int out_dtype, int64_t n,
                             double p, const int64_t* rng, int64_t stream_id, void* stream);
 
@@ -493,8 +494,8 @@ DECIK_API int decik_dropout(const void* x, int x_dtype, const void* residual, vo
  *   da_b = scale_b du_b^T (keep_b x16)                 fp32 [n_branch rank, width], contiguous
  * addend fp32 (ld_add) may be NULL, or dx itself. The sums run in a fixed order: the same inputs give
  * the same bits. workspace: decik_lora_down_dropout_bwd_workspace() bytes, 16-byte aligned.
- * width % 8 == 0; rank % 8 == 0, the branches' ranks rounded up to 16 together <= 64; rows and
- * pointers 16-byte aligned. */
+ * n_tok <= 2^24; width % 8 == 0; rank % 8 == 0, the branches' ranks rounded up to 16 together <= 64;
+ * rows and pointers 16-byte aligned. */
 DECIK_API int decik_lora_down_dropout(const void* x, int x_dtype, int64_t ldx, const void* a, int64_t lda, void* x16,
                                       int64_t ldx16, void* u, int64_t ldu, int u_cols, int64_t n_tok, int width,
                                       int rank, int n_branch, double p0, double p1, const int64_t* rng, int64_t stream_id,

@@ -42,7 +42,7 @@ def test_axis_of(sections, interleaved, want):
     assert list(ops.rope_axis_of(sections, interleaved)) == want == list(o_rope.axis_of(sections, interleaved))
 
 
-@pytest.mark.parametrize("sections", [(), (1, 1, 1, 1, 1), (4, -1), (2.5, 1)])
+@pytest.mark.parametrize("sections", [(), (1, 1, 1, 1, 1), (4, -1), (2.5, 1), ("a",), None])
 def test_axis_of_refusals(sections):
     with pytest.raises(RuntimeError, match="sections"):
         ops.rope_axis_of(sections)
@@ -84,6 +84,41 @@ def test_lora_oracle_gradient():
         e = np.zeros_like(a)
         e[j, k] = h
         assert abs((loss(x, a + e) - loss(x, a - e)) / (2 * h) - da[j, k]) < 1e-7
+
+
+def test_counter_dropout_switch(monkeypatch):
+    """SKC_COUNTER_DROPOUT: unset or 0 leaves torch's draws, a seed switches the generator on."""
+    from decik_b200 import solution
+    from decik_b200.solution import _state, attn, dropout, mlp, nf4, rmsnorm, varlen
+
+    for m in (attn, mlp, nf4, rmsnorm, varlen):
+        monkeypatch.setattr(m, "patch", lambda *a, **k: None)
+    try:
+        for value, want in ((None, None), ("0", None), ("", None), ("7", 7)):
+            dropout.use_counter_dropout(False)
+            monkeypatch.delenv("SKC_COUNTER_DROPOUT", raising=False)
+            if value is not None:
+                monkeypatch.setenv("SKC_COUNTER_DROPOUT", value)
+            solution.apply()
+            assert _state.STATE.counter_dropout == want
+        streams = dropout.step_streams(torch.device("cpu"))
+        assert streams.streams(2)[1] == 0 and streams.streams(1)[1] == 2 and streams.rng.tolist() == [7, 0]
+        assert dropout.step_streams(torch.device("cpu")).rng.tolist() == [7, dropout.STREAMS]
+        with pytest.raises(RuntimeError, match="more than"):
+            streams.streams(dropout.STREAMS)
+    finally:
+        dropout.use_counter_dropout(False)
+    assert dropout.step_streams(torch.device("cpu")) is None
+
+
+def test_counter_rng_state_is_int64():
+    from decik_b200.solution.dropout import CounterRNG
+
+    for seed in (0, 2 ** 63 + 5, -3, 2 ** 64 - 1):
+        r = CounterRNG(seed, "cpu")
+        assert r.state.tolist()[0] % 2 ** 64 == seed % 2 ** 64
+    a, b = r.take(2), r.take(1)
+    assert a.tolist()[1] == 0 and b.tolist()[1] == 2 and r.state.tolist()[1] == 3
 
 
 # ------------------------------------------------------------------------------------ refusals

@@ -609,6 +609,63 @@ def test_captured_step_draws_new_masks(ops):
             assert torch.equal(a_, b_)
 
 
+def test_captured_training_step(ops):
+    """Forward and backward of the autograd Functions captured once, replayed with the state advancing."""
+    from decik_b200.solution.attn import QKNormRope
+    from decik_b200.solution.dropout import CounterDropout, CounterRNG, LoRADownDropout
+
+    s = _heads_case(96, 4, 2, 64, 64, BF16)
+    leaf = lambda t: t.detach().clone().requires_grad_(True)
+    q, k, wq, wk = (leaf(s[n]) for n in ("q", "k", "wq", "wk"))
+    x, a = leaf(torch.randn(96, 256, device="cuda")), leaf(torch.randn(16, 256, device="cuda"))
+    leaves = [q, k, wq, wk, x, a]
+    r = CounterRNG(4)
+
+    def step():
+        state = r.take(2)
+        oq, ok = QKNormRope.apply(q, None, k, wq, wk, 1e-6, s["cos"], s["sin"])
+        u = LoRADownDropout.apply(CounterDropout.apply(x, 0.3, state, 0), (0.5,), state, 1, BF16, a)
+        return torch.autograd.grad((oq * oq).float().sum() + ok.float().sum() + (u * u).float().sum(), leaves)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(3):
+        r.state.copy_(torch.tensor([4, 10 * i], device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        r.state.copy_(torch.tensor([4, 10 * i], device="cuda"))
+        for g, w in zip(got, step()):
+            assert torch.equal(g, w)
+        if i:
+            assert not torch.equal(got[4], last)
+        last = got[4]
+
+
+def test_binding_argument_errors(ops):
+    """What is no tensor, or not as many arguments, is an error and not a crash."""
+    from decik_b200 import _lib
+
+    x, rng = torch.randn(8, device="cuda"), _rng()
+    with pytest.raises(RuntimeError, match="not a tensor"):
+        ops.dropout([1.0], 0.1, rng)
+    with pytest.raises(RuntimeError, match="arguments instead of"):
+        _lib.bind().dropout(x, 0.1, rng)
+    with pytest.raises((TypeError, RuntimeError)):
+        ops.dropout(x, "a", rng)
+    with pytest.raises(RuntimeError, match="out_dtype"):
+        ops.dropout(x, 0.1, rng, out_dtype=3)
+    with pytest.raises(RuntimeError, match="p for each"):
+        ops.lora_down_dropout(x.view(1, 8), x.view(1, 8).to(BF16), (0.1, 0.1, 0.1), rng)
+
+
 def test_two_streams_at_once(ops):
     s = _heads_case(3000, 12, 2, 128, 128, BF16)
     x, a, du, add = _lora_case(3000, 512, 16, (0.1, 0.1), FP32, BF16)
