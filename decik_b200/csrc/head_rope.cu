@@ -53,13 +53,15 @@ __device__ __forceinline__ float load_w(const void* w, int dtype, int i) {
 
 // cos and sin of position * inv_freq, to fp32's last bits of the exact product's: the quarter turns
 // are counted and taken off in 64 bits (a far position times a 24-bit frequency needs more than 32),
-// so that what is rounded to fp32 is at most an eighth of a turn, exact relative to itself.
+// so that what is rounded to fp32 is at most an eighth of a turn, exact relative to itself. Adding
+// 1.5 2^52 rounds to whole quarters and leaves their count in the sum's low bits (up to 2^51 quarters,
+// beyond which 64 bits hold no angle).
 __device__ __forceinline__ void sincos_of(double pos, float inv_freq, float& s, float& c) {
   const double quarters = pos * static_cast<double>(inv_freq) * 0.63661977236758134;  // 2 / pi
-  const double n = rint(quarters);
-  const int quadrant = static_cast<int>(static_cast<long long>(n) & 3);
+  const double whole = quarters + 6755399441055744.0;
+  const int quadrant = __double2loint(whole);
   float a, b;
-  sincospif(0.5f * static_cast<float>(quarters - n), &a, &b);
+  sincospif(0.5f * static_cast<float>(quarters - (whole - 6755399441055744.0)), &a, &b);
   s = quadrant & 1 ? b : a;
   c = quadrant & 1 ? a : b;
   if (quadrant & 2) s = -s;
