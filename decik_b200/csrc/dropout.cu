@@ -1,7 +1,8 @@
 // Dropout from a counter-based generator (philox.cuh), with no stored mask: out = [residual +]
 // keep * scale * x over n values in row-major order. The same call on the gradient is its backward.
 //
-// HBM-bound: each value is read once and written once, the mask is computed.
+// HBM-bound: each value is read once and written once, the mask is computed. 16,384 x 1536 bf16 added to an
+// fp32 residual: 252 MB in 41.1 us (6.1 TB/s, 0.93 of a plain copy's rate); 830 x 1536 fp16: 2.8 us.
 #include "philox.cuh"
 
 namespace decik {
@@ -40,9 +41,10 @@ __device__ __forceinline__ void store8(O* p, const float (&f)[8]) {
   }
 }
 
-// A thread takes groups of 8 values, kUnroll of them with their loads in flight together. VEC: every
-// pointer is 16-byte aligned; without it, and for the last n % 8 values, one value at a time. Dropped
-// values are 0 whatever x holds there (NaN included).
+// A thread takes groups of 8 values, kUnroll of them with their loads in flight together (the residual
+// case above: 43.4 us with 1, 41.1 with 2, 41.6 with 4). VEC: every pointer is 16-byte aligned; without
+// it (122 us instead of 43 in a stream), and for the last n % 8 values, one value at a time. Dropped values
+// are 0 whatever x holds there (NaN included).
 constexpr int kUnroll = 2;
 
 template <typename X, typename O, bool RES, bool VEC>

@@ -12,7 +12,9 @@
 // All arithmetic is fp32 with one rounding at the end. HBM-bound. L lanes hold a token's row of D values,
 // 16 each, and walk over its heads: the angles (read from the tables or computed), with the weights
 // folded in, stay in registers for all of them, a row's mean square is log2 L shuffles, and a lane's two
-// 16-byte pieces are rotation partners.
+// 16-byte pieces are rotation partners. Norms and tables at 131,072 tokens, 28 / 4 heads of 128: 343 us for
+// 2.28 GB, a plain copy's rate; three axes at 16,384 tokens, 12 / 2 heads: 20.0 us for 118 MB (5.9 TB/s);
+// norm backward there: 37.3 us for 193 MB (5.2 TB/s).
 #include "common.cuh"
 #include "ptx.cuh"
 
@@ -183,7 +185,8 @@ constexpr int kThreads = 128;
 
 // Forward; with sign -1 and without norms also the backward (the rotation by the opposite angle).
 // Block (x, y): 128 / L tokens, heads y * per_group .. of the queries' and then the keys' heads. The
-// loads of U heads are in flight together.
+// loads of U heads are in flight together: 343 us at 131,072 tokens with 4, 494 with 2, 361 with 8; with
+// a LoRA delta, which doubles the loads, 10.3 us at 4,099 tokens with 2, 11.7 with 1, 15.7 with 4.
 template <typename T, int L, bool NORM, bool AXES, bool LORA>
 __global__ void __launch_bounds__(kThreads) fwd_kernel(const Args p, int w_dtype, int per_group, float sign) {
   constexpr int U = LORA ? 2 : 4;
@@ -305,6 +308,8 @@ __device__ __forceinline__ uint4 pack_f2(const f2* x) {
 // registers (kept in a slot in shared memory while the warp is at the other part, queries or keys),
 // then the CTA's lanes that hold the same values, then the CTAs in a kernel of their own, all in a
 // fixed order.
+// Two rows ahead take 37.1 us at 16,384 tokens of 12 / 2 heads, three 37.6; a tile a CTA at a time, with a
+// row ahead in registers, took 48.2.
 constexpr int kDepth = 3, kSlot = 20;  // kSlot: floats of a lane's slot, 16 and padding against bank conflicts
 
 template <int L, bool LORA>
@@ -521,7 +526,9 @@ constexpr int kMaxPart = 2048;  // CTAs of a backward pass with norms
 template <typename T, int L>
 int launch_fwd_l(const Args& p, bool norm, bool axes, int w_dtype, float sign, cudaStream_t s) {
   const int64_t tiles = (p.n_tok + kThreads / L - 1) / (kThreads / L);
-  // few tokens: the heads of a token over several CTAs, until there are four for every SM
+  // Few tokens: the heads of a token over several CTAs, until there are four for every SM. At 2,000 tokens
+  // of 12 / 2 heads that takes 4.1 us, up to 6, 8 and 12 for every SM 5.6, 5.7 and 7.2 (the angles are
+  // computed again in each); at 10,000 of 16 / 4 heads of 64 12.9 against 14.0, 12.7 and 12.4.
   const int heads = p.hq + p.hk;
   int64_t groups = 4 * static_cast<int64_t>(sm_count()) / tiles;
   groups = groups < 1 ? 1 : groups > heads ? heads : groups;
