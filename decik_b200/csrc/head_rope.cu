@@ -449,34 +449,40 @@ __global__ void __launch_bounds__(kThreads, LORA ? 3 : 4) norm_bwd_kernel(const 
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = add2(v[i], yv[i]);
       }
-      f2 ss0 = mul2(v[0], v[0]), ss1 = mul2(v[1], v[1]);
+      // Both sums in one round of shuffles: of x^2, and of z w x with x as it was read (the mean needs it
+      // times r, which the first sum gives).
+      f2 ss0 = mul2(v[0], v[0]), ss1 = mul2(v[1], v[1]), zx0 = 0ull, zx1 = 0ull;  // two zeros each
+      f2 d[8];
+      const ulonglong2* const w = reinterpret_cast<const ulonglong2*>(ws + (part * L + c) * kSlot);
 #pragma unroll
       for (int i = 2; i < 8; i += 2) {
         ss0 = fma2(v[i], v[i], ss0);
         ss1 = fma2(v[i + 1], v[i + 1], ss1);
       }
-      // (of a row that is not there 0, so that it adds nothing to the sums with eps = 0 either)
-      const float rs = rsqrtf(row_sum<L>(sum2(add2(ss0, ss1))) * inv_d + p.eps), r = t < n_tok ? rs : 0.f;
-      const f2 rr = pack2f(r, r);
-      f2 zx0 = 0ull, zx1 = 0ull;  // two zeros each
-      const ulonglong2* const w = reinterpret_cast<const ulonglong2*>(ws + (part * L + c) * kSlot);
 #pragma unroll
       for (int i = 0; i < 8; i += 2) {
         const ulonglong2 wv = w[i / 2];
-        v[i] = mul2(v[i], rr);
-        v[i + 1] = mul2(v[i + 1], rr);
-        const f2 d0 = mul2(z[i], v[i]), d1 = mul2(z[i + 1], v[i + 1]);
-        dw[i] = add2(dw[i], d0);
-        dw[i + 1] = add2(dw[i + 1], d1);
-        zx0 = fma2(d0, wv.x, zx0);
-        zx1 = fma2(d1, wv.y, zx1);
+        d[i] = mul2(z[i], v[i]);
+        d[i + 1] = mul2(z[i + 1], v[i + 1]);
+        zx0 = fma2(d[i], wv.x, zx0);
+        zx1 = fma2(d[i + 1], wv.y, zx1);
         z[i] = mul2(z[i], wv.x);
         z[i + 1] = mul2(z[i + 1], wv.y);
       }
-      const float mean = -row_sum<L>(sum2(add2(zx0, zx1))) * inv_d;
-      const f2 mm = pack2f(mean, mean);
+      float ss = sum2(add2(ss0, ss1)), zx = sum2(add2(zx0, zx1));
 #pragma unroll
-      for (int i = 0; i < 8; ++i) z[i] = mul2(rr, fma2(v[i], mm, z[i]));
+      for (int o = L / 2; o > 0; o >>= 1) {
+        ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        zx += __shfl_xor_sync(0xffffffffu, zx, o);
+      }
+      // (of a row that is not there 0, so that it adds nothing to the sums with eps = 0 either)
+      const float rs = rsqrtf(ss * inv_d + p.eps), r = t < n_tok ? rs : 0.f, mean = -(r * r) * (zx * inv_d);
+      const f2 rr = pack2f(r, r), mm = pack2f(mean, mean);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        dw[i] = fma2(d[i], rr, dw[i]);
+        z[i] = mul2(rr, fma2(v[i], mm, z[i]));
+      }
       if (ok) {
         stg16(dst, pack_f2<T>(z));
         stg16(dst + up, pack_f2<T>(z + 4));
@@ -503,20 +509,23 @@ __global__ void __launch_bounds__(kThreads, LORA ? 3 : 4) norm_bwd_kernel(const 
   }
 }
 
-// dw[d] = the sum of the CTAs' partials in a fixed order: thread (d, j) of a block sums CTAs j, j + 32, ...
-// for one of its 32 values, then the 32 sums are added in order.
+// dw[d] = the sum of the CTAs' partials in a fixed order: thread (d, j) of a block sums CTAs j, j + 64, ...
+// for one of its 16 values, then the 64 sums are added as a tree.
 __global__ void __launch_bounds__(1024) dw_sum_kernel(const float* __restrict__ part, float* __restrict__ dwq,
                                                       float* __restrict__ dwk, int n_part, int D) {
-  __shared__ float red[32][33];
-  const int d = blockIdx.x * 32 + (threadIdx.x & 31), j = threadIdx.x >> 5;  // 2 D is a multiple of 32
+  __shared__ float red[64][17];
+  const int i = threadIdx.x & 15, d = blockIdx.x * 16 + i, j = threadIdx.x >> 4;  // D is a multiple of 16
   float s = 0.f;
 #pragma unroll 8
-  for (int c = j; c < n_part; c += 32) s += __ldg(part + static_cast<int64_t>(c) * 2 * D + d);
-  red[j][threadIdx.x & 31] = s;
+  for (int c = j; c < n_part; c += 64) s += __ldg(part + static_cast<int64_t>(c) * 2 * D + d);
+  red[j][i] = s;
   __syncthreads();
-  if (j != 0) return;
-  for (int k = 1; k < 32; ++k) s += red[k][threadIdx.x];
-  (d < D ? dwq : dwk)[d < D ? d : d - D] = s;
+#pragma unroll
+  for (int w = 32; w > 0; w >>= 1) {
+    if (j < w) red[j][i] += red[j + w][i];
+    __syncthreads();
+  }
+  if (j == 0) (d < D ? dwq : dwk)[d < D ? d : d - D] = red[0][i];
 }
 
 int lanes_of(int D) { return D <= 64 ? 4 : D <= 128 ? 8 : 16; }
@@ -670,7 +679,7 @@ int run_bwd(const char* what, Args p, bool axes, int w_dtype, float* dwq, float*
   p.part = static_cast<float*>(workspace);
   int n_part = 0;
   if (int rc = DECIK_DISPATCH_16(dtype, [&] { return launch_bwd<T>(p, axes, w_dtype, &n_part, s); })) return rc;
-  dw_sum_kernel<<<2 * p.D / 32, 1024, 0, s>>>(p.part, dwq, dwk, n_part, p.D);
+  dw_sum_kernel<<<2 * p.D / 16, 1024, 0, s>>>(p.part, dwq, dwk, n_part, p.D);
   return check_launch(what);
 }
 

@@ -222,8 +222,8 @@ class _PackedStep:
         self.packing = packing
 
     def __enter__(self):
+        STATE.dropout = step_streams(self.packing.index.device)  # first: it may raise
         STATE.packing, STATE.packing_active = self.packing, True
-        STATE.dropout = step_streams(self.packing.index.device)
         return self.packing
 
     def __exit__(self, *exc):
