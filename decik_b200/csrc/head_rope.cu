@@ -14,7 +14,7 @@
 // folded in, stay in registers for all of them, a row's mean square is log2 L shuffles, and a lane's two
 // 16-byte pieces are rotation partners. Norms and tables at 131,072 tokens, 28 / 4 heads of 128: 343 us for
 // 2.28 GB, a plain copy's rate; three axes at 16,384 tokens, 12 / 2 heads: 20.0 us for 118 MB (5.9 TB/s);
-// norm backward there: 37.3 us for 193 MB (5.2 TB/s).
+// norm backward there: 36.9 us for 193 MB (5.2 TB/s; the pass itself 6 TB/s, then the weights' gradients).
 #include "common.cuh"
 #include "ptx.cuh"
 
@@ -560,7 +560,9 @@ int launch_bwd_k(const Args& p, int w_dtype, int* n_part, cudaStream_t s) {
   auto kernel = norm_bwd_kernel<T, L, AXES, LORA>;
   if (int rc = ensure_dyn_smem(kernel, bwd_smem<L, LORA>(), done, "head_rope_bwd")) return rc;
   const int64_t rows = (p.n_tok + 32 / L - 1) / (32 / L) * (p.hq + p.hk);
-  int64_t ctas = static_cast<int64_t>(sm_count()) * (LORA ? 3 : 4);  // all that run at once
+  // All CTAs that run at once, however few rows each warp then has: 830 tokens of 12 / 2 heads take 8.1 us, with
+  // at least 6 rows a warp 8.5, with 12 10.8; 5,050 of 3 / 3 heads 12.1, 11.6, 13.7.
+  int64_t ctas = static_cast<int64_t>(sm_count()) * (LORA ? 3 : 4);
   if (ctas > kMaxPart) ctas = kMaxPart;
   const int64_t warps = ctas * (kThreads / 32), per_warp = (rows + warps - 1) / warps;
   const int64_t used = (rows + per_warp - 1) / per_warp;
