@@ -175,6 +175,31 @@ def test_lora_down_dropout_bwd(ops, T, W, rank, p, xd, dt, with_addend):
     assert torch.equal(dx, dx2) and torch.equal(da, da2)        # fixed order of the sums
 
 
+def test_lora_long_batch_keeps_its_precision(ops):
+    """40,000 tokens. dA is summed in chunks of at most 1,024 tokens on the tensor cores, then 40 chunks in
+    fp32, so the count of its roundings stops growing with the batch at 1024 of 2^-23 and 40 of 2^-24 of the
+    sum of the magnitudes; a warp of the forward sums W / 8 products, and the 8 warps' sums are added. 8 more
+    of each for the scale, as above. The reference runs in 64 bits on the GPU with the mask of ops.dropout."""
+    T, W, rank, p = 40000, 3584, 16, (0.1, 0.4)
+    x, a, du, add = _lora_case(T, W, rank, p, BF16, BF16)
+    dx, da = ops.lora_down_dropout_bwd(du, x, a, p, _rng(), 1, addend=add)
+    _, u = ops.lora_down_dropout(x, a, p, _rng(), 1)
+    ones = torch.ones(T, W, device="cuda")
+    want_dx, mag_dx = add.double(), add.double().abs()
+    for b in range(2):
+        rows = slice(rank * b, rank * (b + 1))
+        keep = ops.dropout(ones, p[b], _rng(), 1 + b).double()
+        xm, g, ab = x.double() * keep, du[:, rows].double(), a[rows].double()
+        mag = g.abs().T @ xm.abs()
+        assert ((da[rows].double() - g.T @ xm).abs() <= (1024 * U23 + 40 * U24 + 8 * U23) * mag).all()
+        want, mag = xm @ ab.T, xm.abs() @ ab.abs().T
+        bound = (W / 8 + 8 + 8) * U23 * mag
+        assert ((u[:, rows].double() - want).abs() <= bound + torch.finfo(BF16).eps / 2 * (want.abs() + bound)).all()
+        want_dx += keep * (g @ ab)
+        mag_dx += keep * (g.abs() @ ab.abs())
+    assert ((dx.double() - want_dx).abs() <= (2 * rank + 8) * U23 * mag_dx).all()
+
+
 def test_lora_gradients_are_the_forwards_differences(ops):
     """dA and dx against differences of the forward's u (fp32 differences of a 16-bit u: a linear
     function, so a large step is exact up to u's roundings)."""
