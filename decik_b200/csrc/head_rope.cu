@@ -639,6 +639,8 @@ int set_axes(const char* what, Args& p, const void* positions, int pos_dtype, in
                      pos_dtype);
   if (!axis_of || (p.n_tok != 0 && (!positions || !inv_freq)) || (n_axes > 1 && ld_pos < p.n_tok))
     return set_error(DECIK_ERR_INVALID, "%s: null pointer, or rows of positions shorter than the tokens", what);
+  if (p.n_tok != 0 && !aligned16(inv_freq))  // load_angles reads it in 16-byte pieces
+    return set_error(DECIK_ERR_INVALID, "%s: inv_freq is not 16-byte aligned", what);
   p.ang.pos = positions;
   p.ang.pos32 = pos_dtype;
   p.ang.n_axes = n_axes;

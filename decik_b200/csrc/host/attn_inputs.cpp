@@ -16,6 +16,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cstdint>
 #include <initializer_list>
 #include <optional>
 #include <stdexcept>
@@ -149,11 +150,11 @@ int tables(const char* what, const Tensor& cos, const Tensor& sin, int64_t T) {
 }
 
 struct Axes {
-  Tensor positions;  // as they are passed
+  Tensor positions, inv_freq;  // as they are passed
   int pos_dtype, n_axes, R;
   int64_t ld_pos;
-  const float* inv_freq;
   const uint8_t* axis_of;
+  const float* inv_freq_ptr() const { return static_cast<const float*>(inv_freq.data_ptr()); }
 };
 // axis_of: bytes, the axis of each frequency; n_axes sections
 Axes axes(const Args& a, int i_pos, int i_inv, int i_map, int i_axes, int64_t T) {
@@ -175,7 +176,8 @@ Axes axes(const Args& a, int i_pos, int i_inv, int i_map, int i_axes, int64_t T)
   const Tensor& inv = a.tensor(i_inv);
   if (inv.scalar_type() != at::kFloat || inv.dim() != 1 || inv.size(0) != n || !inv.is_contiguous())
     fail(a.what, "inv_freq must be contiguous fp32 [sum(sections)]");
-  x.inv_freq = static_cast<const float*>(inv.data_ptr());
+  // a slice of a longer table may start anywhere; the kernels read 16-byte pieces
+  x.inv_freq = reinterpret_cast<uintptr_t>(inv.data_ptr()) % 16 == 0 ? inv : inv.clone();
   x.axis_of = reinterpret_cast<const uint8_t*>(map);
   x.R = static_cast<int>(2 * n);
   return x;
@@ -264,8 +266,8 @@ PyObject* rope_axes_fwd(PyObject*, PyObject* const* v, Py_ssize_t n) {
   check(decik_rope_axes_fwd(h.q.v, h.lora, h.k.v, ptr(wq), ptr(wk),
                             wq == nullptr ? DECIK_F32 : code(a.what, wq->scalar_type()),
                             static_cast<float>(a.number(8)), x.positions.data_ptr(), x.pos_dtype, x.ld_pos, x.n_axes,
-                            x.inv_freq, x.axis_of, out_view(oq, h.D, h.T * h.D), out_view(ok, h.D, h.T * h.D), h.T, h.Hq,
-                            h.Hk, h.D, x.R, code(a.what, q.scalar_type()), at.stream),
+                            x.inv_freq_ptr(), x.axis_of, out_view(oq, h.D, h.T * h.D), out_view(ok, h.D, h.T * h.D),
+                            h.T, h.Hq, h.Hk, h.D, x.R, code(a.what, q.scalar_type()), at.stream),
         a.what);
   return wrap({oq, ok});
   END_HANDLE_TH_ERRORS
@@ -293,7 +295,7 @@ PyObject* rope_axes_bwd(PyObject*, PyObject* const* v, Py_ssize_t n) {
   const HeadOuts o = head_outs(gq, h.T, h.Hq, h.Hk, h.D, norm);
   check(decik_rope_axes_bwd(g.q.v, g.k.v, h.q.v, h.lora, h.k.v, ptr(wq), ptr(wk),
                             norm ? code(a.what, wq->scalar_type()) : DECIK_F32, static_cast<float>(a.number(10)),
-                            x.positions.data_ptr(), x.pos_dtype, x.ld_pos, x.n_axes, x.inv_freq, x.axis_of,
+                            x.positions.data_ptr(), x.pos_dtype, x.ld_pos, x.n_axes, x.inv_freq_ptr(), x.axis_of,
                             out_view(o.dq, int64_t(h.Hq) * h.D, h.D), out_view(o.dk, int64_t(h.Hk) * h.D, h.D),
                             norm ? static_cast<float*>(o.dwq.data_ptr()) : nullptr,
                             norm ? static_cast<float*>(o.dwk.data_ptr()) : nullptr, h.T, h.Hq, h.Hk, h.D, x.R,

@@ -520,8 +520,8 @@ DECIK_API int decik_lora_down_dropout_bwd(const void* du, int64_t ld_du, const v
  * decik_qk_norm_rope_*: cos, sin fp32 [n_tok, rotary_dim], 16-byte aligned; both norm weights.
  * decik_rope_axes_*: the angle of frequency j < R / 2 is positions[axis_of[j]][t] * inv_freq[j], reduced in
  * 64 bits; positions int64 (pos_dtype 0) or int32 (1) [n_axes, n_tok] with rows ld_pos apart, inv_freq
- * fp32 [R / 2] on the device, axis_of a HOST array of R / 2 bytes (each < n_axes <= 4), read during the
- * call; the norm weights both given or both NULL.
+ * fp32 [R / 2] on the device, 16-byte aligned, axis_of a HOST array of R / 2 bytes (each < n_axes <= 4), read
+ * during the call; the norm weights both given or both NULL.
  * Backward, from grad_q / grad_k and the forward's inputs (q, q_lora, k are read only with norms):
  *   dq, dk  views of dtype (dq is the gradient of q and of q_lora)
  *   dq_weight, dk_weight  fp32 [head_dim], written whole (with norms), summed in a fixed order;

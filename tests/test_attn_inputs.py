@@ -232,6 +232,20 @@ def test_axes_refusals():
     assert fwd(n=0) == 0
 
 
+@pytest.mark.parametrize("bwd", [False, True])
+def test_axes_refuse_an_unaligned_inv_freq(bwd):
+    """The kernels read the frequencies in 16-byte pieces: a pointer to the middle of one is refused."""
+    tail = (P, 0, 4, 3, ODD, bytes([0, 1, 2, 0] * 16))
+    end = (4, 2, 1, 128, 128, 1)
+    lib = _lib.lib()
+    if bwd:
+        rc = lib.decik_rope_axes_bwd(_v(), _v(), _v(), NONE3, _v(), P, P, 2, 1e-6, *tail, _v(), _v(), P, P, *end, None,
+                                     None)  # (without a workspace: refused after this check, so that it never runs)
+    else:
+        rc = lib.decik_rope_axes_fwd(_v(), NONE3, _v(), None, None, 2, 1e-6, *tail, _v(), _v(), *end, None)
+    _refused(rc, b"inv_freq is not 16-byte aligned")
+
+
 def test_ops_refuse_cpu_tensors():
     q, k = torch.zeros(4, 2, 64, dtype=torch.bfloat16), torch.zeros(4, 1, 64, dtype=torch.bfloat16)
     w, cs, rng = torch.ones(64), torch.ones(4, 64), torch.zeros(2, dtype=torch.int64)

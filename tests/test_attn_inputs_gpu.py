@@ -458,6 +458,23 @@ def test_rope_axes_position_views(ops):
     assert all(torch.equal(x, y) for x, y in zip(a, b))
 
 
+@pytest.mark.parametrize("normed", [False, True])
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_rope_axes_inv_freq_slices(ops, off, normed):
+    """inv_freq as a slice of a longer table, wherever it starts: the same bits."""
+    s = _heads_case(40, 4, 2, 64, 64, BF16)
+    table = torch.rand(40, generator=_gen(3), device="cuda")
+    pos = torch.randint(0, 999, (3, 40), generator=_gen(4), device="cuda")
+    part = table[off:off + 32]
+    assert part.data_ptr() % 16 == 4 * off
+    norm = dict(q_weight=s["wq"], k_weight=s["wk"], eps=s["eps"]) if normed else {}
+    saved = dict(norm, q=s["q"], k=s["k"]) if normed else {}
+    run = lambda inv: (ops.rope_axes_fwd(s["q"], s["k"], pos, inv, (16, 8, 8), **norm)
+                       + ops.rope_axes_bwd(s["gq"], s["gk"], pos, inv, (16, 8, 8), **saved))
+    for a, b in zip(run(part), run(part.clone())):
+        assert torch.equal(a, b)
+
+
 def test_heads_empty(ops):
     s = _heads_case(4, 2, 1, 64, 64, BF16)
     args = (s["q"][:0], s["k"][:0], s["wq"], s["wk"], s["eps"], s["cos"][:0], s["sin"][:0])
