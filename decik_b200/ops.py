@@ -650,12 +650,27 @@ def qkv_proj_fwd(x: torch.Tensor, w_cat: torch.Tensor, ext_b: torch.Tensor, lora
 def qkv_proj_gemm(x16: torch.Tensor, u: torch.Tensor, w_cat: torch.Tensor, ext_b: torch.Tensor, cos: torch.Tensor,
                   sin: torch.Tensor, n_heads: int, n_kv: int):
     """q [Hq, T, D], k [Hk, T, D], v [T, Hk, D] of qkv_proj_fwd from a caller's x16 [T, H] and u [T, 64]
-    (u_q | u_v | 1 | zeros, lora_down_dropout's with u_cols 64): its GEMM alone (decik_qkv_proj_gemm)."""
-    _cuda(x16, u, w_cat, ext_b, cos, sin)
+    (u_q | u_v | 1 | zeros, lora_down_dropout's with u_cols 64): its GEMM alone (decik_qkv_proj_gemm).
+    w_cat [(Hq+2Hk)*D, H] (its rows behind these are not read) and ext_b [(Hq+2Hk)*D, 64] of x16's
+    dtype, cos and sin fp32 [T, D]."""
+    if x16.dim() != 2 or x16.dtype not in (torch.float16, torch.bfloat16) or cos.dim() != 2:
+        raise RuntimeError("decik_b200 qkv_proj_gemm: x16 fp16 / bf16 [T, H], cos and sin [T, D]")
     T, H = x16.shape
-    D = cos.shape[-1]
-    if u.shape != (T, 4 * LORA_RANK) or not u.is_contiguous() or x16.stride(1) != 1 or w_cat.stride(1) != 1:
-        raise RuntimeError("decik_b200 qkv_proj_gemm: u contiguous [T, 64], x16 and w_cat with contiguous rows")
+    D = cos.shape[1]
+    n_proj, wide = (n_heads + 2 * n_kv) * D, 4 * LORA_RANK
+    if not u.dtype == w_cat.dtype == ext_b.dtype == x16.dtype:
+        raise RuntimeError("decik_b200 qkv_proj_gemm: u, w_cat and ext_b must have x16's dtype")
+    if u.shape != (T, wide) or not u.is_contiguous() or x16.stride(1) != 1:
+        raise RuntimeError("decik_b200 qkv_proj_gemm: u contiguous [T, 64], x16 with contiguous rows")
+    if w_cat.dim() != 2 or w_cat.shape[0] < n_proj or w_cat.shape[1] != H or w_cat.stride(1) != 1:
+        raise RuntimeError(f"decik_b200 qkv_proj_gemm: w_cat must be [{n_proj}, {H}] with contiguous rows")
+    if ext_b.dim() != 2 or ext_b.shape[0] < n_proj or ext_b.shape[1] != wide or not ext_b.is_contiguous():
+        raise RuntimeError(f"decik_b200 qkv_proj_gemm: ext_b must be contiguous [{n_proj}, {wide}]")
+    if cos.shape != sin.shape or cos.shape[0] < T or not cos.dtype == sin.dtype == torch.float32:
+        raise RuntimeError("decik_b200 qkv_proj_gemm: cos and sin must be fp32 [T, D]")
+    _cuda(x16, u, w_cat, ext_b, cos, sin)
+    if any(t.device != x16.device for t in (u, w_cat, ext_b, cos, sin)):
+        raise RuntimeError("decik_b200 qkv_proj_gemm: tensors must be on one CUDA device")
     q = torch.empty((n_heads, T, D), dtype=x16.dtype, device=x16.device)
     k = torch.empty((n_kv, T, D), dtype=x16.dtype, device=x16.device)
     v = torch.empty((T, n_kv, D), dtype=x16.dtype, device=x16.device)

@@ -246,6 +246,28 @@ def test_axes_refuse_an_unaligned_inv_freq(bwd):
     _refused(rc, b"inv_freq is not 16-byte aligned")
 
 
+@pytest.mark.parametrize("change,text", [
+    (dict(u=lambda t: t[:3]), "u contiguous"), (dict(u=lambda t: t[:, :32]), "u contiguous"),
+    (dict(u=lambda t: t.half()), "dtype"), (dict(w_cat=lambda t: t.half()), "dtype"),
+    (dict(ext_b=lambda t: t.half()), "dtype"), (dict(x16=lambda t: t.float()), "x16 fp16"),
+    (dict(x16=lambda t: t[0]), "x16 fp16"), (dict(w_cat=lambda t: t[:511]), "w_cat must be"),
+    (dict(w_cat=lambda t: t[:, :128]), "w_cat must be"), (dict(w_cat=lambda t: t.t().contiguous().t()), "w_cat must be"),
+    (dict(ext_b=lambda t: t[:511]), "ext_b must be"), (dict(ext_b=lambda t: t[:, :32]), "ext_b must be"),
+    (dict(ext_b=lambda t: t.repeat(1, 2)[:, :64]), "ext_b must be"),
+    (dict(cos=lambda t: t[:3], sin=lambda t: t[:3]), "cos and sin"), (dict(sin=lambda t: t[:3]), "cos and sin"),
+    (dict(cos=lambda t: t.half()), "cos and sin"), (dict(sin=lambda t: t.double()), "cos and sin"),
+    (dict(cos=lambda t: t[0]), "cos and sin"), ({}, "CUDA device")])
+def test_qkv_proj_gemm_refusals(change, text):
+    """Operands of another type or with too few rows, refused on the host before anything is read."""
+    T, H, Hq, Hk = 4, 256, 2, 1     # 512 rows of projections
+    args = dict(x16=torch.zeros(T, H, dtype=torch.bfloat16), u=torch.zeros(T, 64, dtype=torch.bfloat16),
+                w_cat=torch.zeros(544, H, dtype=torch.bfloat16), ext_b=torch.zeros(512, 64, dtype=torch.bfloat16),
+                cos=torch.zeros(T, 128), sin=torch.zeros(T, 128))
+    args = {n: change.get(n, lambda t: t)(t) for n, t in args.items()}
+    with pytest.raises(RuntimeError, match=text):
+        ops.qkv_proj_gemm(**args, n_heads=Hq, n_kv=Hk)
+
+
 def test_ops_refuse_cpu_tensors():
     q, k = torch.zeros(4, 2, 64, dtype=torch.bfloat16), torch.zeros(4, 1, 64, dtype=torch.bfloat16)
     w, cs, rng = torch.ones(64), torch.ones(4, 64), torch.zeros(2, dtype=torch.int64)
