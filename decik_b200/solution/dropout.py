@@ -90,11 +90,15 @@ class CounterDropout(torch.autograd.Function):
 class LoRADownDropout(torch.autograd.Function):
     """The LoRA down projections of x [T, W] under dropout, u [T, branches * rank] =
     scale_b (keep_b x16) A_b^T with a mask for each branch (ops.lora_down_dropout). ``a``: the branches'
-    lora_A weights [rank, W] (fp32, as peft keeps them), ``p`` the probability of each, ``dtype`` the
-    compute dtype. Keeps the 16-bit input only."""
+    lora_A weights [rank, W] (fp32, as peft keeps them), of one rank, ``p`` the probability of each (a
+    number: the same for all), ``dtype`` the compute dtype. Keeps the 16-bit input only."""
 
     @staticmethod
     def forward(ctx, x, p, rng, stream, dtype, *a):
+        p = tuple(p) if isinstance(p, (tuple, list)) else (p,) * len(a)
+        if not 1 <= len(a) <= 2 or len(p) != len(a) or any(w.dim() != 2 or w.shape != a[0].shape for w in a):
+            raise RuntimeError(f"decik_b200 LoRADownDropout: {len(p)} probabilities for lora_A weights of shapes "
+                               f"{[tuple(w.shape) for w in a]} (1 or 2 weights [rank, W] of one rank, a p for each)")
         a16 = torch.cat(a).to(dtype)
         x16, u = ops.lora_down_dropout(x if x.dtype == dtype else x.float(), a16, p, rng, stream)
         ctx.save_for_backward(x16, a16, rng)

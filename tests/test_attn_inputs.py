@@ -121,6 +121,17 @@ def test_counter_rng_state_is_int64():
     assert a.tolist()[1] == 0 and b.tolist()[1] == 2 and r.state.tolist()[1] == 3
 
 
+@pytest.mark.parametrize("p,ranks", [((0.1, 0.3), (8, 24)), ((0.1, 0.3), (16,)), ((0.1,), (16, 16)), ((), (16,)),
+                                     (0.1, (8, 8, 8)), (0.1, ()), ([0.1, 0.1, 0.1], (8, 8)), (0.1, (8, 16))])
+def test_lora_down_dropout_function_wants_a_p_for_each_weight(p, ranks):
+    """Weights of different ranks, or a number of p's that is not theirs, would get one another's masks."""
+    from decik_b200.solution.dropout import LoRADownDropout
+
+    a = [torch.zeros(r, 64) for r in ranks]
+    with pytest.raises(RuntimeError, match="LoRADownDropout"):
+        LoRADownDropout.apply(torch.zeros(4, 64), p, torch.zeros(2, dtype=torch.int64), 0, torch.bfloat16, *a)
+
+
 # ------------------------------------------------------------------------------------ refusals
 P = ctypes.c_void_p(256)   # never dereferenced: the checks fail before any CUDA call
 ODD = ctypes.c_void_p(260)

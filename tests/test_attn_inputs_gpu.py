@@ -617,6 +617,24 @@ def test_autograd_functions_match_the_oracle(ops):
     _check(torch.cat([w.grad for w in a]), wda, mda, 48, "da", U23)
 
 
+@pytest.mark.parametrize("p", [0.3, (0.3, 0.3), [0.3, 0.3]], ids=["number", "tuple", "list"])
+def test_lora_down_dropout_function_gives_each_weight_its_mask(ops, p):
+    """One p for two weights: two branches with masks of their own, as in the oracle, both ways."""
+    from decik_b200.solution.dropout import LoRADownDropout
+
+    x, a, du, _ = _lora_case(40, 64, 24, (0.3, 0.3), FP32, BF16)
+    x.requires_grad_(True)
+    ws = [w.float().requires_grad_(True) for w in a.split(24)]
+    u = LoRADownDropout.apply(x, p, _rng(), 1, BF16, *ws)
+    u.backward(du)
+    x16 = _np(x.to(BF16))
+    want, mag = o_drop.lora_down(x16, _np(a), (0.3, 0.3), 3, 2 ** 33 + 5, 1)
+    _check(u, want, mag, 64 + 8, "u", U23)
+    wdx, wda, mdx, mda = o_drop.lora_down_bwd(_np(du), x16, _np(a), (0.3, 0.3), 3, 2 ** 33 + 5, 1)
+    _check(x.grad, wdx, mdx, 24 + 8, "dx", U23)
+    _check(torch.cat([w.grad for w in ws]), wda, mda, 40 + 8, "da", U23)
+
+
 def test_captured_step_draws_new_masks(ops):
     """One captured forward and backward: replays read the generator's state from the device."""
     from decik_b200.solution.dropout import CounterRNG
