@@ -15,6 +15,8 @@
 // 16-byte pieces are rotation partners. Norms and tables at 131,072 tokens, 28 / 4 heads of 128: 343 us for
 // 2.28 GB, a plain copy's rate; three axes at 16,384 tokens, 12 / 2 heads: 20.0 us for 118 MB (5.9 TB/s);
 // norm backward there: 36.9 us for 193 MB (5.2 TB/s; the pass itself 6 TB/s, then the weights' gradients).
+#include <type_traits>
+
 #include "common.cuh"
 #include "ptx.cuh"
 
@@ -186,8 +188,13 @@ constexpr int kThreads = 128;
 // Forward; with sign -1 and without norms also the backward (the rotation by the opposite angle).
 // Block (x, y): 128 / L tokens, heads y * per_group .. of the queries' and then the keys' heads. The
 // loads of U heads are in flight together: 343 us at 131,072 tokens with 4, 494 with 2, 361 with 8; with
-// a LoRA delta, which doubles the loads, 10.3 us at 4,099 tokens with 2, 11.7 with 1, 15.7 with 4.
-template <typename T, int L, bool NORM, bool AXES, bool LORA>
+// a LoRA delta, which doubles the loads, 10.4 us at 4,099 tokens with 2, 11.7 with 1, 15.7 with 4.
+// PART: R < D. A value behind R is no partner of another, and a sine of 0 would not keep an infinity or a NaN
+// there from it (0 inf is NaN), so its partner's share is left out: by a select of each value without norms
+// (6.8 us instead of 6.5 at 4,099 tokens of 14 / 2 heads of 80, none of it at 16,384 of 12 / 2 of 128). With norms
+// the selects took 28.6 us instead of 24.3 at 16,384 of 12 / 2 of 128 (R = 64), a branch on the lane as much; there
+// only a row with an infinity comes to that (its r is 0, and 0 inf is NaN), which is read again: 24.7 us.
+template <typename T, int L, bool NORM, bool AXES, bool LORA, bool PART>
 __global__ void __launch_bounds__(kThreads) fwd_kernel(const Args p, int w_dtype, int per_group, float sign) {
   constexpr int U = LORA ? 2 : 4;
   const Lane l = lane_of(threadIdx.x % L, p.D, p.R);
@@ -210,9 +217,9 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(const Args p, int w_dtype
     for (int i = 0; i < 8; ++i) {
       const int hi = AXES ? i : 8 + i;
       m[0][i] = NORM ? w[i] * cs[i] : cs[i];
-      m[1][i] = sign * (NORM ? w[8 + i] * sn[i] : sn[i]);
+      m[1][i] = PART && !l.rot ? 0.f : sign * (NORM ? w[8 + i] * sn[i] : sn[i]);
       m[2][i] = NORM ? w[8 + i] * cs[hi] : cs[hi];
-      m[3][i] = sign * (NORM ? w[i] * sn[hi] : sn[hi]);
+      m[3][i] = PART && !l.rot ? 0.f : sign * (NORM ? w[i] * sn[hi] : sn[hi]);
     }
     const T* src = static_cast<const T*>(in.ptr) + t * in.tok_stride + first * in.head_stride;
     const T* lora = LORA && !part ? static_cast<const T*>(p.ql.ptr) + t * p.ql.tok_stride + first * p.ql.head_stride : src;
@@ -220,6 +227,7 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(const Args p, int w_dtype
     T* dst = static_cast<T*>(out.ptr) + t * out.tok_stride + first * out.head_stride;
     for (int h = first; h < last; h += U) {
       Raw raw[U], rl[LORA ? U : 1];
+      unsigned infinite = 0u;  // a bit for each row whose r is 0, in lanes behind R
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         raw[u] = load_raw(src + u * in.head_stride, l, ok && h + u < last);
@@ -241,10 +249,26 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(const Args p, int w_dtype
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          o[i] = x[i] * m[0][i] - x[8 + i] * m[1][i];
-          o[8 + i] = x[8 + i] * m[2][i] + x[i] * m[3][i];
+          o[i] = x[i] * m[0][i] - (PART && !NORM && !l.rot ? 0.f : x[8 + i]) * m[1][i];
+          o[8 + i] = x[8 + i] * m[2][i] + (PART && !NORM && !l.rot ? 0.f : x[i]) * m[3][i];
         }
-        if (ok) store(dst + u * out.head_stride, l, o);
+        const bool later = NORM && PART && !l.rot && r == 0.f;
+        if constexpr (NORM && PART) infinite |= (later ? 1u : 0u) << u;
+        if (ok && !later) store(dst + u * out.head_stride, l, o);
+      }
+      if constexpr (NORM && PART) {
+        if (infinite != 0u && ok) {  // values behind R of rows with an infinity, each alone
+#pragma unroll 1
+          for (int u = 0; u < U; ++u) {
+            if (!(infinite >> u & 1u)) continue;
+            float x[16];
+            unpack<T>(load_raw(src + u * in.head_stride, l, true), x);
+            if constexpr (LORA) add<T>(load_raw(lora + u * lora_hs, l, !part), x);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = x[i] * 0.f * (i < 8 ? m[0][i & 7] : m[2][i & 7]);
+            store(dst + u * out.head_stride, l, x);
+          }
+        }
       }
       src += U * in.head_stride;
       lora += U * lora_hs;
@@ -309,7 +333,8 @@ __device__ __forceinline__ uint4 pack_f2(const f2* x) {
 // then the CTA's lanes that hold the same values, then the CTAs in a kernel of their own, all in a
 // fixed order.
 // Two rows ahead take 37.1 us at 16,384 tokens of 12 / 2 heads, three 37.6; a tile a CTA at a time, with a
-// row ahead in registers, took 48.2.
+// row ahead in registers, took 48.2. PART as in the forward, by selects (10,007 tokens of 16 / 4 heads of 64, R =
+// 32: 22.0 us instead of 21.6).
 constexpr int kDepth = 3, kSlot = 20;  // kSlot: floats of a lane's slot, 16 and padding against bank conflicts
 
 template <int L, bool LORA>
@@ -317,7 +342,7 @@ constexpr int bwd_smem() {
   return kThreads * kDepth * (LORA ? 6 : 4) * 16 + (2 * kThreads + 2 * L) * kSlot * 4;
 }
 
-template <typename T, int L, bool AXES, bool LORA>
+template <typename T, int L, bool AXES, bool LORA, bool PART>
 __global__ void __launch_bounds__(kThreads, LORA ? 3 : 4) norm_bwd_kernel(const Args p, int w_dtype, int64_t n_rows, int64_t per_warp) {
   constexpr int P = LORA ? 6 : 4, TOK = 32 / L;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -436,8 +461,8 @@ __global__ void __launch_bounds__(kThreads, LORA ? 3 : 4) norm_bwd_kernel(const 
         unpack_f2<T>(*reinterpret_cast<const uint4*>(got + kThreads * 16), gv + 4);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          z[i] = fma2(gv[i], cl[i], mul2(gv[4 + i], sh[i]));
-          z[4 + i] = fma2(gv[4 + i], AXES ? cl[i] : ch[AXES ? 0 : i], mul2(gv[i], nsl[i]));
+          z[i] = fma2(gv[i], cl[i], mul2(!PART || l.rot ? gv[4 + i] : 0ull, sh[i]));
+          z[4 + i] = fma2(gv[4 + i], AXES ? cl[i] : ch[AXES ? 0 : i], mul2(!PART || l.rot ? gv[i] : 0ull, nsl[i]));
         }
       }
       unpack_f2<T>(*reinterpret_cast<const uint4*>(got + 2 * kThreads * 16), v);
@@ -545,19 +570,23 @@ int launch_fwd_l(const Args& p, bool norm, bool axes, int w_dtype, float sign, c
   const dim3 grid(static_cast<unsigned>(tiles), (heads + per_group - 1) / per_group);
   auto go = [&](auto kernel) { kernel<<<grid, kThreads, 0, s>>>(p, w_dtype, per_group, sign); };
   const bool lora = p.ql.ptr != nullptr;
-  if (norm) {
-    if (axes) lora ? go(fwd_kernel<T, L, true, true, true>) : go(fwd_kernel<T, L, true, true, false>);
-    else lora ? go(fwd_kernel<T, L, true, false, true>) : go(fwd_kernel<T, L, true, false, false>);
-  } else {
-    lora ? go(fwd_kernel<T, L, false, true, true>) : go(fwd_kernel<T, L, false, true, false>);
-  }
+  auto pick = [&](auto part) {
+    constexpr bool P = decltype(part)::value;
+    if (norm) {
+      if (axes) lora ? go(fwd_kernel<T, L, true, true, true, P>) : go(fwd_kernel<T, L, true, true, false, P>);
+      else lora ? go(fwd_kernel<T, L, true, false, true, P>) : go(fwd_kernel<T, L, true, false, false, P>);
+    } else {
+      lora ? go(fwd_kernel<T, L, false, true, true, P>) : go(fwd_kernel<T, L, false, true, false, P>);
+    }
+  };
+  if (p.R < p.D) pick(std::true_type()); else pick(std::false_type());
   return check_launch("head_rope_fwd");
 }
 
-template <typename T, int L, bool AXES, bool LORA>
+template <typename T, int L, bool AXES, bool LORA, bool PART>
 int launch_bwd_k(const Args& p, int w_dtype, int* n_part, cudaStream_t s) {
   static std::atomic<unsigned long long> done{0};
-  auto kernel = norm_bwd_kernel<T, L, AXES, LORA>;
+  auto kernel = norm_bwd_kernel<T, L, AXES, LORA, PART>;
   if (int rc = ensure_dyn_smem(kernel, bwd_smem<L, LORA>(), done, "head_rope_bwd")) return rc;
   const int64_t rows = (p.n_tok + 32 / L - 1) / (32 / L) * (p.hq + p.hk);
   // All CTAs that run at once, however few rows each warp then has: 830 tokens of 12 / 2 heads take 8.1 us, with
@@ -575,10 +604,14 @@ int launch_bwd_k(const Args& p, int w_dtype, int* n_part, cudaStream_t s) {
 template <typename T, int L>
 int launch_bwd_l(const Args& p, bool axes, int w_dtype, int* n_part, cudaStream_t s) {
   const bool lora = p.ql.ptr != nullptr;
-  if (axes) return lora ? launch_bwd_k<T, L, true, true>(p, w_dtype, n_part, s)
-                        : launch_bwd_k<T, L, true, false>(p, w_dtype, n_part, s);
-  return lora ? launch_bwd_k<T, L, false, true>(p, w_dtype, n_part, s)
-              : launch_bwd_k<T, L, false, false>(p, w_dtype, n_part, s);
+  auto pick = [&](auto part) {
+    constexpr bool P = decltype(part)::value;
+    if (axes) return lora ? launch_bwd_k<T, L, true, true, P>(p, w_dtype, n_part, s)
+                          : launch_bwd_k<T, L, true, false, P>(p, w_dtype, n_part, s);
+    return lora ? launch_bwd_k<T, L, false, true, P>(p, w_dtype, n_part, s)
+                : launch_bwd_k<T, L, false, false, P>(p, w_dtype, n_part, s);
+  };
+  return p.R < p.D ? pick(std::true_type()) : pick(std::false_type());
 }
 
 template <typename T>

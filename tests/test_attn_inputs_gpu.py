@@ -458,6 +458,75 @@ def test_rope_axes_position_views(ops):
     assert all(torch.equal(x, y) for x, y in zip(a, b))
 
 
+BEHIND = [(80, 48, BF16), (64, 32, FP16), (256, 16, BF16), (112, 96, FP16)]   # D, R, dtype
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("lora", [False, True])
+@pytest.mark.parametrize("D,R,dt", BEHIND)
+def test_values_behind_the_rotated_ones_stay_apart(ops, D, R, dt, lora, bad):
+    """An infinity or NaN behind rotary_dim comes out at its own place, and every other value of the row, and
+    of the gradient through the plain rotation, keeps its bits."""
+    T, H = 21, 2
+    s = _heads_case(T, H, 1, D, R, dt, lora=lora)
+    pos, inv = torch.randint(0, 999, (2, T), generator=_gen(4), device="cuda"), torch.rand(R // 2, device="cuda")
+    sections = (R // 2 - 3, 3)
+    for d in sorted({R, R + 3, R + 8, D - 9, D - 1}):
+        if d < R:
+            continue
+        q, gq = s["q"].clone(), s["gq"].clone()
+        q[5, 1, d] = gq[1, 5, d] = bad
+        fwd = lambda q: ops.rope_axes_fwd(q, s["k"], pos, inv, sections, q_lora=s["ql"])
+        bwd = lambda g: ops.rope_axes_bwd(g, s["gk"], pos, inv, sections)
+        for got, want in ((fwd(q)[0].transpose(0, 1), fwd(s["q"])[0].transpose(0, 1)), (bwd(gq)[0], bwd(s["gq"])[0])):
+            assert torch.equal(torch.nan_to_num(got[5, 1, d], nan=7.0), torch.nan_to_num(torch.tensor(
+                bad, dtype=dt, device="cuda"), nan=7.0))
+            got[5, 1, d] = want[5, 1, d]
+            assert torch.equal(got, want), d
+
+
+@pytest.mark.parametrize("axes", [False, True])
+@pytest.mark.parametrize("D,R,dt", BEHIND)
+def test_normed_values_behind_the_rotated_ones_stay_apart(ops, D, R, dt, axes):
+    """The same with norms: a weight's NaN reaches its own place of each row alone, an infinity of x makes the
+    row's other values 0 (the mean is infinite), a gradient's infinity leaves the sums of the other
+    weights' gradients as they were."""
+    T, H = 40, 3
+    s = _heads_case(T, H, 1, D, R, dt)
+    pos, inv = torch.randint(0, 999, (2, T), generator=_gen(4), device="cuda"), torch.rand(R // 2, device="cuda")
+    sections, inf = (R // 2 - 3, 3), float("inf")
+    for d in sorted({R, R + 3, R + 8, D - 9, D - 1}):
+        if d < R:
+            continue
+
+        def fwd(q, wq):
+            if axes:
+                return ops.rope_axes_fwd(q, s["k"], pos, inv, sections, q_weight=wq, k_weight=s["wk"], eps=1e-6)[0]
+            return ops.qk_norm_rope_fwd(q, s["k"], wq, s["wk"], 1e-6, s["cos"], s["sin"])[0]
+
+        def dwq(gq):
+            if axes:
+                return ops.rope_axes_bwd(gq, s["gk"], pos, inv, sections, q=s["q"], k=s["k"], q_weight=s["wq"],
+                                         k_weight=s["wk"], eps=1e-6)[2]
+            return ops.qk_norm_rope_bwd(gq, s["gk"], s["q"], s["k"], s["wq"], s["wk"], 1e-6, s["cos"], s["sin"])[2]
+
+        rest = [i for i in range(D) if i != d]
+        want, w = fwd(s["q"], s["wq"]), s["wq"].clone()
+        w[d] = float("nan")
+        got = fwd(s["q"], w)
+        assert torch.isnan(got[..., d]).all() and torch.equal(got[..., rest], want[..., rest])
+        q = s["q"].clone()
+        q[5, 1, d] = inf
+        got = fwd(q, s["wq"])
+        assert torch.isnan(got[1, 5, d]) and not got[1, 5, rest].any()
+        got[1, 5] = want[1, 5]
+        assert torch.equal(got, want)
+        want, gq = dwq(s["gq"]), s["gq"].clone()
+        gq[1, 5, d] = inf
+        got = dwq(gq)
+        assert not torch.isfinite(got[d]) and torch.equal(got[rest], want[rest])
+
+
 @pytest.mark.parametrize("normed", [False, True])
 @pytest.mark.parametrize("off", [1, 2, 3])
 def test_rope_axes_inv_freq_slices(ops, off, normed):
