@@ -18,6 +18,7 @@ import torch.nn.functional as F
 from .. import ops
 from . import rmsnorm
 from ._state import STATE, on_gpu
+from .dropout import LoRADownDropout
 
 # keyword under which the patched decoder layer hands its input RMSNorm to the patched attention
 INPUT_NORM_KW = "decik_input_norm"
@@ -326,6 +327,25 @@ def _lora_pair(x, link, parts_q, parts_v, packing, dtype):
                                   parts_q[2], parts_v[2], parts_q[3], parts_v[3], packed, dtype)
 
 
+def _lora_counter(x, parts_q, parts_v, dtype):
+    """The q and v LoRA deltas of the normed input x [1, T, W] under the packed step's counter-based
+    dropout (dropout.LoRADownDropout: no mask, no masked copy of x), or None for a width or ranks that
+    its kernels are not for."""
+    width, parts = x.shape[-1], (parts_q, parts_v)
+    ranks = [a.shape[0] for a, _, _, _ in parts]
+    if width % 8 != 0 or any(r % 8 != 0 or r > 64 for r in ranks):
+        return None
+    rows = x.reshape(-1, width)
+    rng, stream = STATE.dropout.streams(2)
+    if ranks[0] == ranks[1] and ranks[0] <= 32:
+        u = LoRADownDropout.apply(rows, (parts_q[3], parts_v[3]), rng, stream, dtype, parts_q[0], parts_v[0])
+        us = u.split(ranks[0], 1)
+    else:  # a pass each
+        us = [LoRADownDropout.apply(rows, p, rng, stream + i, dtype, a) for i, (a, _, _, p) in enumerate(parts)]
+    return [(F.linear(u, b.to(dtype)) * scaling).view(x.shape[:-1] + (b.shape[0],))
+            for u, (_, b, scaling, _) in zip(us, parts)]
+
+
 def _single_lora(layer, lora_cls):
     """The active adapter name of a plain (unmerged) LoRA layer, else None (solution/attn.py:326-341)."""
     try:
@@ -484,15 +504,25 @@ def patch(recompute_lora=True, linear4bit_cls=None, lora_classes=None, fused_blo
         if (recompute_lora and link is not None and link[0] is x
                 and isinstance(link[1], torch.Tensor) and link[1].shape == x.shape):
             parts_q, parts_v = _lora_parts(self.q_proj, q_name), _lora_parts(self.v_proj, v_name)
+        counter = None
+        if STATE.dropout is not None:
+            # the counter-based generator: the branches here, or (None) through their dropout modules,
+            # which draw from it too
+            counter_parts = [_lora_parts(m, n) for m, n in ((self.q_proj, q_name), (self.v_proj, v_name))]
+            if None not in counter_parts and any(p[3] > 0.0 for p in counter_parts):
+                parts_q = parts_v = None
+                counter = _lora_counter(x, *counter_parts, dtype)
         # same call order as the base (q, k, v): the LoRA dropout draws stay in step
         q_base = self.q_proj.base_layer(x.to(dtype))
-        if parts_q is None or parts_v is None:
+        if counter is not None:
+            q_lora, v_lora = counter
+        elif parts_q is None or parts_v is None:
             q_lora = _lora_delta(self.q_proj, q_name, x)
         k = self.k_proj(x.to(dtype))
         v_base = self.v_proj.base_layer(x.to(dtype))
-        if parts_q is None or parts_v is None:
+        if counter is None and (parts_q is None or parts_v is None):
             v_lora = _lora_delta(self.v_proj, v_name, x)
-        else:
+        elif counter is None:
             q_lora, v_lora = _lora_pair(x, link, parts_q, parts_v, packing, dtype)
         v = (v_base.float() + v_lora.float()).to(dtype)
         q_rot, k_rot = FusedQKRope.apply(

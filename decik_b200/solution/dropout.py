@@ -62,10 +62,11 @@ def step_streams(device):
 def use_counter_dropout(on=True) -> None:
     """Switch the packed path's dropout to the counter-based generator: ``True`` (seeded by
     torch.initial_seed()) or a seed; False switches back to torch's draws. Dropout on the packed
-    decoder (nn.Dropout, and the LoRA branches of the fused attention block, which then takes layers with
-    LoRA dropout too) draws at the real tokens only, stores no mask, and does not touch torch's
-    generators. Each packed forward takes new streams. Ranks of a data-parallel job give different
-    seeds."""
+    decoder (nn.Dropout with 0 < p < 1 and not in place, and the LoRA branches of the attention: in the
+    fused block, which then takes layers with LoRA dropout too, in LoRADownDropout for the layers and
+    ranks that the block is not for, in their nn.Dropout for what that is not for) draws at the real
+    tokens only, stores no mask, and does not touch torch's generators. Each packed forward takes new
+    streams. Ranks of a data-parallel job give different seeds."""
     STATE.counter_dropout = None if on is False or on is None else on
     STATE.counter_rngs = {}
 
