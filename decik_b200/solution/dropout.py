@@ -26,11 +26,13 @@ class CounterRNG:
     def __init__(self, seed: int | None = None, device="cuda"):
         seed = torch.initial_seed() if seed is None else int(seed)
         seed = (seed + 2 ** 63) % 2 ** 64 - 2 ** 63  # as int64
-        self.state = torch.tensor([seed, 0], dtype=torch.int64, device=device)
+        with torch.inference_mode(False):  # a state made in an evaluation serves the training after it
+            self.state = torch.tensor([seed, 0], dtype=torch.int64, device=device)
 
     def take(self, n: int = 1) -> torch.Tensor:
-        now = self.state.clone()
-        self.state[1] += n
+        with torch.inference_mode(False):
+            now = self.state.clone()
+            self.state[1] += n
         return now
 
 

@@ -121,6 +121,34 @@ def test_counter_rng_state_is_int64():
     assert a.tolist()[1] == 0 and b.tolist()[1] == 2 and r.state.tolist()[1] == 3
 
 
+def test_counter_rng_serves_inference_and_training():
+    """Made or advanced inside inference mode, the state goes on outside it, and what was taken can be saved
+    for a backward pass."""
+    from decik_b200.solution.dropout import CounterRNG
+
+    class Saves(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, state):
+            ctx.save_for_backward(state)
+            return x * 1
+
+        @staticmethod
+        def backward(ctx, grad):
+            return grad, None
+
+    with torch.inference_mode():
+        r = CounterRNG(7, "cpu")
+        first = r.take(3)
+    second = r.take(2)
+    with torch.inference_mode():
+        third = r.take(1)
+    assert [t.tolist() for t in (first, second, third)] == [[7, 0], [7, 3], [7, 5]] and r.state.tolist() == [7, 6]
+    for state in (first, second, third):
+        x = torch.ones(2, requires_grad=True)
+        Saves.apply(x, state).sum().backward()
+        assert x.grad.tolist() == [1, 1]
+
+
 @pytest.mark.parametrize("p,ranks", [((0.1, 0.3), (8, 24)), ((0.1, 0.3), (16,)), ((0.1,), (16, 16)), ((), (16,)),
                                      (0.1, (8, 8, 8)), (0.1, ()), ([0.1, 0.1, 0.1], (8, 8)), (0.1, (8, 16))])
 def test_lora_down_dropout_function_wants_a_p_for_each_weight(p, ranks):
