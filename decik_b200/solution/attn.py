@@ -46,7 +46,7 @@ def _rows16(t):
     """t [A, B, D] as the head kernels read it: D contiguous, pointer and strides 16-byte aligned."""
     ok = (t.stride(2) == 1 and t.data_ptr() % 16 == 0
           and all(t.shape[i] == 1 or t.stride(i) % 8 == 0 for i in (0, 1)))
-    return t if ok else t.contiguous()
+    return t if ok else t.clone(memory_format=torch.contiguous_format)  # (also of a contiguous one that starts off 16)
 
 
 class QKNormRope(torch.autograd.Function):

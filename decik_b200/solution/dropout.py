@@ -90,6 +90,15 @@ class CounterDropout(torch.autograd.Function):
         return ops.dropout(grad, p, rng, stream, out_dtype=dtype), None, None, None, grad if residual else None
 
 
+def _rows(t):
+    """t [T, W] as the LoRA kernels read it: contiguous rows that start on 16 bytes, one behind the other."""
+    if t.dim() != 2:
+        return t
+    ok = (t.stride(1) == 1 and t.data_ptr() % 16 == 0
+          and (t.shape[0] == 1 or (t.stride(0) >= t.shape[1] and t.stride(0) * t.element_size() % 16 == 0)))
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
 class LoRADownDropout(torch.autograd.Function):
     """The LoRA down projections of x [T, W] under dropout, u [T, branches * rank] =
     scale_b (keep_b x16) A_b^T with a mask for each branch (ops.lora_down_dropout). ``a``: the branches'
@@ -103,7 +112,7 @@ class LoRADownDropout(torch.autograd.Function):
             raise RuntimeError(f"decik_b200 LoRADownDropout: {len(p)} probabilities for lora_A weights of shapes "
                                f"{[tuple(w.shape) for w in a]} (1 or 2 weights [rank, W] of one rank, a p for each)")
         a16 = torch.cat(a).to(dtype)
-        x16, u = ops.lora_down_dropout(x if x.dtype == dtype else x.float(), a16, p, rng, stream)
+        x16, u = ops.lora_down_dropout(_rows(x if x.dtype == dtype else x.float()), a16, p, rng, stream)
         ctx.save_for_backward(x16, a16, rng)
         ctx.meta = (p, stream, x.dtype, [w.dtype for w in a])
         return u
@@ -112,6 +121,6 @@ class LoRADownDropout(torch.autograd.Function):
     def backward(ctx, du):
         x16, a16, rng = ctx.saved_tensors
         p, stream, x_dtype, a_dtypes = ctx.meta
-        dx, da = ops.lora_down_dropout_bwd(du.contiguous(), x16, a16, p, rng, stream)
+        dx, da = ops.lora_down_dropout_bwd(_rows(du), x16, a16, p, rng, stream)
         parts = da.split(da.shape[0] // len(a_dtypes))
         return (dx.to(x_dtype), None, None, None, None) + tuple(w.to(t) for w, t in zip(parts, a_dtypes))

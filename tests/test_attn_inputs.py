@@ -149,6 +149,30 @@ def test_counter_rng_serves_inference_and_training():
         assert x.grad.tolist() == [1, 1]
 
 
+def test_functions_align_their_rows():
+    """A contiguous tensor that starts off a 16-byte boundary is copied, as are strides that the kernels
+    refuse; what they take is passed as it is."""
+    from decik_b200.solution.attn import _rows16
+    from decik_b200.solution.dropout import _rows
+
+    buf = torch.arange(4 * 2 * 16 + 3, dtype=torch.bfloat16)
+    assert buf.data_ptr() % 16 == 0
+    for off in (1, 3):
+        t = buf[off:off + 128].view(4, 2, 16)
+        for got, want in ((_rows16(t), t), (_rows(t.view(8, 16)), t.view(8, 16)), (_rows16(t[:1]), t[:1])):
+            assert got.data_ptr() % 16 == 0 and got.is_contiguous() and torch.equal(got, want)
+    wide = torch.arange(8 * 20.0).view(8, 20)
+    for t in (wide[:, 1:17], wide[:1, 2:18].expand(8, 16), wide.bfloat16()[:, 4:20], wide.t(),
+              torch.tensor(2.0).expand(8, 16)):
+        got = _rows(t)
+        assert got.data_ptr() % 16 == 0 and got.is_contiguous() and torch.equal(got, t)
+    for t in (wide[:, 4:], wide, wide.bfloat16().view(4, 40)[:, 8:24], wide[:1, 4:], wide[0]):
+        assert _rows(t) is t
+    heads = buf[:128].view(4, 2, 16)
+    for t in (heads, heads[:, :1], heads[:, :1].expand(4, 3, 16), heads.transpose(0, 1)):
+        assert _rows16(t) is t
+
+
 @pytest.mark.parametrize("p,ranks", [((0.1, 0.3), (8, 24)), ((0.1, 0.3), (16,)), ((0.1,), (16, 16)), ((), (16,)),
                                      (0.1, (8, 8, 8)), (0.1, ()), ([0.1, 0.1, 0.1], (8, 8)), (0.1, (8, 16))])
 def test_lora_down_dropout_function_wants_a_p_for_each_weight(p, ranks):

@@ -704,6 +704,49 @@ def test_lora_down_dropout_function_gives_each_weight_its_mask(ops, p):
     _check(torch.cat([w.grad for w in ws]), wda, mda, 40 + 8, "da", U23)
 
 
+def test_functions_take_tensors_off_16_bytes(ops):
+    """Inputs and gradients that are contiguous but start off a 16-byte boundary (the slices that a cat's
+    backward hands out), and rows of other strides: the aligned tensors' results."""
+    from decik_b200.solution.attn import AxesRope, QKNormRope
+    from decik_b200.solution.dropout import LoRADownDropout
+
+    def off(t):
+        b = torch.empty(t.numel() + 3, dtype=t.dtype, device="cuda")[3:].view(t.shape)
+        assert b.data_ptr() % 16 != 0
+        return b.copy_(t)
+
+    s = _heads_case(20, 4, 2, 64, 64, BF16, lora=True)
+    inv, pos = torch.rand(32, device="cuda"), torch.randint(0, 500, (2, 20), device="cuda")
+    x, a, du, _ = _lora_case(20, 128, 16, (0.3, 0.1), BF16, BF16)
+    first = torch.zeros(3, dtype=BF16, device="cuda")
+    seen = []
+
+    def run(place, join):
+        q, ql, k = (place(s[n]).requires_grad_(True) for n in ("q", "ql", "k"))
+        xx, ws = place(x).requires_grad_(True), [w.float().requires_grad_(True) for w in a.split(16)]
+        u = LoRADownDropout.apply(xx, (0.3, 0.1), _rng(), 1, BF16, *ws)
+        outs = (u, *QKNormRope.apply(q, ql, k, s["wq"], s["wk"], s["eps"], s["cos"], s["sin"]),
+                *AxesRope.apply(q, ql, k, pos, inv, (20, 12)))
+        for o in outs:
+            o.register_hook(lambda g: seen.append(0 if g is None else g.data_ptr() % 16))
+        grads = (du, s["gq"], s["gk"], s["gq"], s["gk"])
+        for o, g in zip(outs, grads):
+            if join:    # the slice of the cat's gradient that goes to o starts 6 bytes behind a boundary
+                torch.cat([first, o.reshape(-1)]).backward(torch.cat([first, g.reshape(-1)]), retain_graph=True)
+            else:
+                o.backward(g.reshape(o.shape), retain_graph=True)
+        return [o.detach() for o in outs] + [t.grad for t in (xx, *ws, q, ql, k)]
+
+    want = run(lambda t: t.detach().clone(memory_format=torch.contiguous_format), False)
+    seen.clear()
+    got = run(off, True)
+    assert 6 in seen
+    assert all(torch.equal(a_, b_) for a_, b_ in zip(got, want))
+    wide = torch.zeros(20, 131, dtype=BF16, device="cuda")
+    wide[:, 3:] = x
+    assert torch.equal(LoRADownDropout.apply(wide[:, 3:], (0.3, 0.1), _rng(), 1, BF16, *a.float().split(16)), want[0])
+
+
 def test_captured_step_draws_new_masks(ops):
     """One captured forward and backward: replays read the generator's state from the device."""
     from decik_b200.solution.dropout import CounterRNG
