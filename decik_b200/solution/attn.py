@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from .. import ops
 from . import rmsnorm
@@ -65,6 +66,7 @@ class QKNormRope(torch.autograd.Function):
         return out_q.unsqueeze(0), out_k.unsqueeze(0)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_q, grad_k):
         q, q_lora, k, wq, wk, cos, sin = ctx.saved_tensors
         dq, dk, dwq, dwk = ops.qk_norm_rope_bwd(_rows16(grad_q[0]), _rows16(grad_k[0]), q, k, wq, wk, ctx.eps, cos,
@@ -90,6 +92,7 @@ class AxesRope(torch.autograd.Function):
         return out_q.unsqueeze(0), out_k.unsqueeze(0)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_q, grad_k):
         q, q_lora, k, wq, wk, positions, inv_freq = ctx.saved_tensors
         sections, interleaved, eps, lora = ctx.meta

@@ -10,6 +10,7 @@ again. Nothing is drawn from torch's generators.
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import ops
 from ._state import STATE
@@ -84,6 +85,7 @@ class CounterDropout(torch.autograd.Function):
         return ops.dropout(x, p, rng, stream, residual=residual)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
         (rng,) = ctx.saved_tensors
         p, stream, dtype, residual = ctx.meta
@@ -118,6 +120,7 @@ class LoRADownDropout(torch.autograd.Function):
         return u
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, du):
         x16, a16, rng = ctx.saved_tensors
         p, stream, x_dtype, a_dtypes = ctx.meta

@@ -747,6 +747,27 @@ def test_functions_take_tensors_off_16_bytes(ops):
     assert torch.equal(LoRADownDropout.apply(wide[:, 3:], (0.3, 0.1), _rng(), 1, BF16, *a.float().split(16)), want[0])
 
 
+def test_second_derivatives_are_refused(ops):
+    """The backward passes are kernels of their own without a derivative: to differentiate them again raises,
+    it does not leave the terms out."""
+    from decik_b200.solution.attn import AxesRope, QKNormRope
+    from decik_b200.solution.dropout import CounterDropout, LoRADownDropout
+
+    s = _heads_case(20, 4, 2, 64, 64, BF16)
+    inv, pos = torch.rand(32, device="cuda"), torch.randint(0, 500, (2, 20), device="cuda")
+    x, a, _, _ = _lora_case(20, 64, 16, (0.3,), FP32, BF16)
+    leaf = lambda t: t.detach().clone().requires_grad_(True)
+    for fn, t in ((lambda t: CounterDropout.apply(t, 0.3, _rng()), x),
+                  (lambda t: LoRADownDropout.apply(t, 0.3, _rng(), 0, BF16, a.float()), x),
+                  (lambda t: QKNormRope.apply(t, None, s["k"], s["wq"], s["wk"], 1e-6, s["cos"], s["sin"])[0], s["q"]),
+                  (lambda t: AxesRope.apply(t, None, s["k"], pos, inv, (20, 12))[0], s["q"])):
+        t = leaf(t)
+        y = fn(t)
+        g, = torch.autograd.grad((y.float() ** 2).sum(), t, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            (g.float().sum() + (t.float() ** 2).sum()).backward()
+
+
 def test_captured_step_draws_new_masks(ops):
     """One captured forward and backward: replays read the generator's state from the device."""
     from decik_b200.solution.dropout import CounterRNG
