@@ -27,6 +27,9 @@ inline int check_launch(const char* what) {
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+// a pointer to values of that many bytes each (a power of two) starts at one
+inline bool aligned_to(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+inline size_t dtype_bytes(int dtype) { return dtype == DECIK_F32 ? 4 : 2; }
 
 // Raises a kernel's dynamic shared-memory limit to `bytes` on the current device, once per device:
 // the setting belongs to each device's context. `done` is the call site's bitmask of devices

@@ -136,6 +136,9 @@ extern "C" int decik_dropout(const void* x, int x_dtype, const void* residual, v
     return set_error(DECIK_ERR_INVALID, "dropout: dtypes %d -> %d are not F16/BF16/F32", x_dtype, out_dtype);
   if (n == 0) return DECIK_OK;
   if (!x || !out || !rng) return set_error(DECIK_ERR_INVALID, "dropout: null pointer");
+  if (!aligned_to(x, dtype_bytes(x_dtype)) || !aligned_to(out, dtype_bytes(out_dtype)) ||
+      !aligned_to(residual, dtype_bytes(out_dtype)) || !aligned_to(rng, 8))
+    return set_error(DECIK_ERR_INVALID, "dropout: a pointer is not aligned to its values");
   cudaStream_t s = as_stream(stream);
   if (x_dtype == DECIK_F32) return launch_x<float>(out_dtype, x, residual, out, n, p, rng, stream_id, s);
   if (x_dtype == DECIK_BF16) return launch_x<__nv_bfloat16>(out_dtype, x, residual, out, n, p, rng, stream_id, s);

@@ -654,6 +654,8 @@ int check(const char* what, const Args& p, bool norm, bool bwd, int w_dtype, int
     ok = ok && view_ok(p.gq.ptr, p.gq.tok_stride, p.gq.head_stride) &&
          view_ok(p.gk.ptr, p.gk.tok_stride, p.gk.head_stride);
   if (!ok) return set_error(DECIK_ERR_INVALID, "%s: a view is NULL, or its pointer or strides are not 16-byte aligned", what);
+  if (norm && (!aligned_to(p.wq, dtype_bytes(w_dtype)) || !aligned_to(p.wk, dtype_bytes(w_dtype))))
+    return set_error(DECIK_ERR_INVALID, "%s: a norm weight is not aligned to its values", what);
   return DECIK_OK;
 }
 
@@ -672,6 +674,8 @@ int set_axes(const char* what, Args& p, const void* positions, int pos_dtype, in
                      pos_dtype);
   if (!axis_of || (p.n_tok != 0 && (!positions || !inv_freq)) || (n_axes > 1 && ld_pos < p.n_tok))
     return set_error(DECIK_ERR_INVALID, "%s: null pointer, or rows of positions shorter than the tokens", what);
+  if (p.n_tok != 0 && !aligned_to(positions, pos_dtype == 1 ? 4 : 8))
+    return set_error(DECIK_ERR_INVALID, "%s: positions are not aligned to their values", what);
   if (p.n_tok != 0 && !aligned16(inv_freq))  // load_angles reads it in 16-byte pieces
     return set_error(DECIK_ERR_INVALID, "%s: inv_freq is not 16-byte aligned", what);
   p.ang.pos = positions;
@@ -699,6 +703,8 @@ int run_bwd(const char* what, Args p, bool axes, int w_dtype, float* dwq, float*
   const bool norm = p.wq != nullptr;
   if (int rc = check(what, p, norm, true, w_dtype, dtype)) return rc;
   if (norm && (!dwq || !dwk)) return set_error(DECIK_ERR_INVALID, "%s: dq_weight or dk_weight NULL", what);
+  if (norm && (!aligned_to(dwq, 4) || !aligned_to(dwk, 4)))
+    return set_error(DECIK_ERR_INVALID, "%s: dq_weight or dk_weight is not aligned to its values", what);
   if (p.n_tok == 0) {
     cudaError_t e = cudaSuccess;
     if (norm) e = cudaMemsetAsync(dwq, 0, sizeof(float) * p.D, s);

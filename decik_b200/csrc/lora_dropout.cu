@@ -557,6 +557,7 @@ extern "C" int decik_lora_down_dropout(const void* x, int x_dtype, int64_t ldx, 
   if (ldx % xe || lda % 8 || (x16 && ldx16 % 8) || ldu % 8 || !aligned16(x) || !aligned16(a) ||
       (x16 && !aligned16(x16)) || !aligned16(u))
     return set_error(DECIK_ERR_INVALID, "lora_down_dropout: rows and pointers need 16-byte alignment");
+  if (!aligned_to(rng, 8)) return set_error(DECIK_ERR_INVALID, "lora_down_dropout: rng is not aligned to its values");
   const DownArgs p{x, ldx, a, lda, x16, ldx16, u, ldu, u_cols, n_tok, width, rank, make_drop(p0, p1), rng, stream_id,
                    as_stream(stream)};
   return DECIK_DISPATCH_16(dtype, [&] {
@@ -591,6 +592,7 @@ extern "C" int decik_lora_down_dropout_bwd(const void* du, int64_t ld_du, const 
   if (ld_du % 8 || ldx % 8 || lda % 8 || ld_dx % 4 || (addend && ld_add % 4) || !aligned16(du) || !aligned16(x16) ||
       !aligned16(a) || !aligned16(dx) || (addend && !aligned16(addend)) || !aligned16(workspace))
     return set_error(DECIK_ERR_INVALID, "lora_down_dropout_bwd: rows and pointers need 16-byte alignment");
+  if (!aligned_to(rng, 8)) return set_error(DECIK_ERR_INVALID, "lora_down_dropout_bwd: rng is not aligned to its values");
   const Drop d = make_drop(p0, p1);
   const Split sp = split_of(n_tok, width);
   const int n_units = sp.n_chunks * sp.col_blocks, n4 = width / 4 * rank * n_branch;

@@ -476,9 +476,9 @@ DECIK_API int decik_mlp_down_grad(const void* grad, int64_t ldg, const void* w_d
  *        that the forward pass saw.
  *
  * decik_dropout: out = keep scale x, or with residual (out's type, may be NULL) residual + keep scale x,
- * over n values; one rounding, to out's type. x, out: F16, BF16 or F32 each, of any alignment; out
- * may be residual, or x where their types are the same. The backward of the dropout is the same call on
- * the gradient. */
+ * over n values; one rounding, to out's type. x, out: F16, BF16 or F32 each, aligned to their values (16-byte
+ * alignment of all three is faster); out may be residual, or x where their types are the same. The
+ * backward of the dropout is the same call on the gradient. */
 DECIK_API int decik_dropout(const void* x, int x_dtype, const void* residual, void* out, int out_dtype, int64_t n,
                             double p, const int64_t* rng, int64_t stream_id, void* stream);
 

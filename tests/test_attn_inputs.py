@@ -331,6 +331,31 @@ def test_qkv_proj_gemm_refusals(change, text):
         ops.qkv_proj_gemm(**args, n_heads=Hq, n_kv=Hk)
 
 
+def test_entries_refuse_pointers_between_values():
+    """A pointer that does not start at a value of its type would be a misaligned access of the kernel."""
+    lib, at = _lib.lib(), lambda n: ctypes.c_void_p(256 + n)
+    text = b"aligned to"
+    drop = lambda x=P, xd=1, res=None, out=P, od=1, rng=P: lib.decik_dropout(x, xd, res, out, od, 8, 0.1, rng, 0, None)
+    for kw in (dict(x=at(1)), dict(x=at(2), xd=2), dict(out=at(1)), dict(out=at(2), od=2), dict(res=at(1)),
+               dict(res=at(2), od=2), dict(rng=at(4))):
+        _refused(drop(**kw), text)
+    _refused(lib.decik_lora_down_dropout(P, 2, 64, P, 64, P, 64, P, 32, 32, 4, 64, 16, 2, 0.1, 0.1, at(4), 0, 1, None), text)
+    _refused(lib.decik_lora_down_dropout_bwd(P, 32, P, 64, P, 64, None, 0, P, 64, P, 4, 64, 16, 2, 0.1, 0.1, at(4), 0, 1,
+                                             P, None), text)
+    norm = lambda wq=P, wk=P, wd=2: lib.decik_qk_norm_rope_fwd(_v(), NONE3, _v(), wq, wk, wd, 1e-6, P, P, _v(), _v(), 4, 2,
+                                                               1, 128, 128, 1, None)
+    for kw in (dict(wq=at(2)), dict(wk=at(2)), dict(wq=at(1), wd=1), dict(wk=at(1), wd=0)):
+        _refused(norm(**kw), text)
+    bwd = lambda dq=P, dk=P: lib.decik_qk_norm_rope_bwd(_v(), _v(), _v(), NONE3, _v(), P, P, 2, 1e-6, P, P, _v(), _v(), dq,
+                                                        dk, 4, 2, 1, 128, 128, 1, P, None)
+    _refused(bwd(dq=at(2)), text)
+    _refused(bwd(dk=at(1)), text)
+    axes = lambda pos, pd: lib.decik_rope_axes_fwd(_v(), NONE3, _v(), None, None, 2, 1e-6, pos, pd, 4, 1, P, bytes(64),
+                                                   _v(), _v(), 4, 2, 1, 128, 128, 1, None)
+    _refused(axes(at(4), 0), text)
+    _refused(axes(at(2), 1), text)
+
+
 def test_ops_refuse_cpu_tensors():
     q, k = torch.zeros(4, 2, 64, dtype=torch.bfloat16), torch.zeros(4, 1, 64, dtype=torch.bfloat16)
     w, cs, rng = torch.ones(64), torch.ones(4, 64), torch.zeros(2, dtype=torch.int64)
