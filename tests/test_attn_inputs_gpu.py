@@ -362,6 +362,31 @@ def test_qk_norm_rope_agrees_with_rope(ops):
         assert (a.float() - b.float()).abs().max() <= 2.0 ** -7     # one bf16 step of values up to 2
 
 
+@pytest.mark.parametrize("T,Hq,Hk,D,dt,lora", [(8003, 12, 2, 128, BF16, False), (8003, 16, 4, 64, FP16, False),
+                                               (3001, 8, 3, 256, BF16, True), (600, 12, 2, 128, BF16, False)])
+def test_norm_weight_gradients_lose_no_part(ops, T, Hq, Hk, D, dt, lora):
+    """The weights' gradients of a batch that fills the GPU, with terms of one sign, so that a partial sum that
+    is lost or counted twice shows. Roundings: a warp's rows of one part in a chain (at most its share of all
+    rows), the CTA's lanes that hold the same values, the CTAs in 64 chains and a tree of 6; each term has
+    those of r (the mean of D squares) and a few products."""
+    s = _heads_case(T, Hq, Hk, D, D, dt, lora=lora)
+    s["cos"], s["sin"] = torch.ones(T, D, device="cuda"), torch.zeros(T, D, device="cuda")
+    for n in "qk":
+        x = s[n].float() + (s["ql"].float() if n == "q" and lora else 0.0)
+        s["g" + n] = (s["g" + n].float().abs() * torch.sign(x).transpose(0, 1)).to(dt).contiguous()
+    got = ops.qk_norm_rope_bwd(s["gq"], s["gk"], s["q"], s["k"], s["wq"], s["wk"], s["eps"], s["cos"], s["sin"],
+                               q_lora=s["ql"])
+    lanes = 4 if D <= 64 else 8 if D <= 128 else 16
+    ctas = torch.cuda.get_device_properties(0).multi_processor_count * (3 if lora else 4)
+    rows = -(-T * lanes // 32) * (Hq + Hk)
+    chain = -(-rows // (4 * ctas)) + 128 // lanes + -(-ctas // 64) + 6
+    for n, dw in zip("qk", got[2:]):
+        g, x = s["g" + n].transpose(0, 1).double(), torch.as_tensor(_x(s, n), device="cuda")
+        want = (g * x * torch.rsqrt((x * x).mean(-1, keepdim=True) + s["eps"])).sum((0, 1)).cpu().numpy()
+        assert (want > 0).all()
+        _check(dw, want, want, chain + D + 32, "dw" + n)
+
+
 def test_qk_norm_rope_views(ops):
     """Head-major and padded inputs, broadcast gradients, one row."""
     s = _heads_case(33, 4, 2, 64, 32, BF16)
