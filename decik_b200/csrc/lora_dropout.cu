@@ -6,10 +6,12 @@
 // The index of x[t, k] is t * width + k (width % 8 == 0: a group of 8 stays in one row).
 //
 // At 16,384 x 1536, fp32 x, bf16, rank 16 x 2: forward 33.0 us (152 MB, 4.6 TB/s), backward 49.7 us (253 MB,
-// 5.1 TB/s). The bytes alone would take 23.2 and 38.6 us; the other bound is the generator, 50 M mask
-// bits each way: its 14 products a call keep the multipliers 64 % busy in the forward, the masks' logic
-// the ALU 53 % in both. mma.sync is far from its limit (rank 32: 10 and 13 %), so the tensor cores of the
-// larger kind would change nothing.
+// 5.1 TB/s). The bytes alone would take 23.2 and 38.6 us. No unit is full: the generator's 14 products a call
+// (50 M mask bits each way) keep the multipliers 64 % busy in the forward, the masks' logic the ALU 53 % in both,
+// issue slots 59 and 58 %, DRAM 70 and 78 %; what is left is latency, with 16 and 14 warps an SM (the ring
+// and the registers allow no more). mma.sync is far from its limit (rank 32: 10 and 13 %), so the tensor cores
+// of the larger kind would change nothing. Ranks above 16 are further from the bytes: rank 32 x 2 takes 50.9 us
+// forward and 65.1 backward (23.4 and 38.8), rank 64 44.1 and 58.7; 830 rows are 52 CTAs for 148 SMs.
 #include <type_traits>
 
 #include "philox.cuh"

@@ -244,7 +244,9 @@ def _bound(what: str, launches: int, *args):
 
 def rope_axis_of(sections, interleaved: bool = False) -> bytes:
     """The axis of each rotary frequency: ``sections[a]`` frequencies of axis a, one block after the
-    other, or ``interleaved``: the axes in turn (0, 1, 2, 0, ...) while they have some left."""
+    other, or ``interleaved``: the axes in turn (0, 1, 2, 0, ...) while they have some left, an axis that has
+    none left being passed over. With (24, 20, 20) or (11, 11, 10) that is also the order that puts axis a > 0 at a,
+    a + 3, ... and axis 0 everywhere else; with sections further apart, such as (24, 22, 18), it is not."""
     try:
         return _axis_of(tuple(map(operator.index, sections)), bool(interleaved))
     except TypeError:
@@ -270,7 +272,8 @@ def qk_norm_rope_fwd(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k
                      cos: torch.Tensor, sin: torch.Tensor, q_lora: torch.Tensor | None = None):
     """RMSNorm of each query and key head (over its D values, with the weights [D]) and RoPE of its first
     cos.shape[1] dims in one pass (decik_qk_norm_rope_fwd). q, k: [T, H, D] views of fp16 / bf16 (D
-    contiguous, 16-byte aligned strides); ``q_lora`` is added to q first; cos, sin fp32 [T, rotary_dim].
+    contiguous, 16-byte aligned strides); ``q_lora`` is added to q first; cos, sin fp32 [T, rotary_dim],
+    16-byte aligned.
     Returns q [Hq, T, D], k [Hk, T, D] head-major, as rope_fwd does."""
     return _bound("qk_norm_rope_fwd", 1, q, k, q_weight, k_weight, eps, cos, sin, q_lora)
 
@@ -290,8 +293,8 @@ def rope_axes_fwd(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv
     """RoPE by positions of several axes (decik_rope_axes_fwd): the angle of frequency j is
     positions[axis of j] * inv_freq[j], computed in the kernel (no cos / sin tables). positions int64 or
     int32 [axes, T] (or [T] for one axis), inv_freq fp32 [R / 2], ``sections`` the number of frequencies
-    of each axis (rope_axis_of), R / 2 = their sum a multiple of 8. With ``q_weight`` and ``k_weight`` each head is normed first, as in
-    qk_norm_rope_fwd. q, k, q_lora and the results as there."""
+    of each axis (rope_axis_of), R / 2 = their sum a multiple of 8. With ``q_weight`` and ``k_weight`` each
+    head is normed first, as in qk_norm_rope_fwd. q, k, q_lora and the results as there."""
     return _bound("rope_axes_fwd", 1, q, k, positions, inv_freq, rope_axis_of(sections, interleaved), len(sections),
                   q_weight, k_weight, eps, q_lora)
 
@@ -331,7 +334,8 @@ def lora_down_dropout(x: torch.Tensor, a: torch.Tensor, p, rng: torch.Tensor, st
                       u_cols: int | None = None):
     """The LoRA down projections of x [T, W] (fp32, or a's dtype) under counter-based dropout
     (decik_lora_down_dropout): a [branches * rank, W] of fp16 / bf16 holds the branches' lora_A, ``p``
-    the probability of each (a number or a tuple); branch b has the mask of (rng, stream + b) over x.
+    the probability of each (a tuple; a number: one branch); branch b has the mask of (rng, stream + b) over
+    x. Rows of x and a start on 16 bytes.
     Returns x16 = x in a's dtype (x itself where it has it) and u [T, branches * rank] =
     scale_b (keep_b x16) A_b^T; with ``u_cols`` (64 for qkv_proj_gemm) u has that many columns, a 1 and
     zeros behind the branches'."""
